@@ -1,0 +1,364 @@
+// Gated linear recurrence (per channel, no counterpart in the reference): the
+// diagonal member of the family that GDN-2 belongs to, on the same layouts and
+// gates,
+//     h_t = e^{g_t} h_{t-1} + w_t v_t,   o_t = h_t,   h_0 given,
+// and its backward pass.  With c_t the gradient that leaves token t towards
+// t-1, c_{T+1} = dh_final,
+//     dh_t = dout_t + c_{t+1},   c_t = e^{g_t} dh_t,
+//     dv_t = w_t dh_t,  dw_t = v_t dh_t,  dg_t = e^{g_t} h_{t-1} dh_t,  dh0 = c_1.
+// Both directions are scans of maps x -> a x + b, joined by
+//     (a2, b2) o (a1, b1) = (a2 a1, a2 b1 + b2).
+//
+// A CTA takes a tile of 64 tokens x 64 channels: 8 warps of 8 tokens, a lane
+// holds 2 neighbouring channels, so a warp reads whole 64-value groups of a
+// row.  A thread folds its 8 tokens, the warps join their maps through shared
+// memory, and each thread walks its tokens again from the state that reaches
+// it: every global byte moves once.  What moves bounds the kernels: float32
+// 16 bytes a value forward, 28 backward.
+//
+// The forward keeps the state that enters each tile (1/64 of o).  The backward
+// rebuilds the states inside a tile from it, so it does not read o; with int8
+// checkpoints it does so from the 8-bit v and w, which makes its gradients
+// those of the restored values, restarted from the true state every 64 tokens.
+// Decays stay in their own type: a rounding of a log decay compounds over the
+// sequence, one of v or w does not.
+#include "../../include/gdn2.h"
+#include "gdn2_int8.cuh"
+
+namespace gdn2 {
+int report_error(int code, const char* msg);
+}
+
+using namespace gdn2;
+
+namespace {
+
+constexpr int kRows = 8;                 // tokens a thread holds
+constexpr int kWarps = 8;
+constexpr int kTile = kRows * kWarps;    // tokens of a tile: the interval of the kept states
+static_assert(kTile == GDN2_RECUR_INTERVAL, "interval of the kept states");
+
+// Two neighbouring channels.
+__device__ __forceinline__ float2 ld2(const float* p) { return __ldcs(reinterpret_cast<const float2*>(p)); }
+__device__ __forceinline__ float2 ld2(const __nv_bfloat16* p) {
+  const unsigned u = __ldcs(reinterpret_cast<const unsigned*>(p));
+  return make_float2(__uint_as_float(u << 16), __uint_as_float(u & 0xffff0000u));
+}
+__device__ __forceinline__ float2 ld2(const int8_t* p) {
+  const short u = __ldcs(reinterpret_cast<const short*>(p));
+  return make_float2((float)(int8_t)(u & 0xff), (float)(int8_t)(u >> 8));
+}
+__device__ __forceinline__ void st2(float* p, float2 v) { __stcs(reinterpret_cast<float2*>(p), v); }
+__device__ __forceinline__ void st2(__nv_bfloat16* p, float2 v) {
+  const __nv_bfloat162 h = __floats2bfloat162_rn(v.x, v.y);
+  __stcs(reinterpret_cast<unsigned*>(p), *reinterpret_cast<const unsigned*>(&h));
+}
+
+// e^g, or from the pre-activation x of g = -softplus(x): sigmoid(-x), from
+// e^{-|x|} so that neither end overflows or cancels.
+__device__ __forceinline__ float sig_from(float e, bool high) { return (high ? 1.f : e) / (1.f + e); }
+__device__ __forceinline__ float decay(float g, int raw) {
+  return raw ? sig_from(expf(-fabsf(g)), g < 0.f) : expf(g);
+}
+__device__ __forceinline__ float2 decay2(float2 g, int raw) {
+  return make_float2(decay(g.x, raw), decay(g.y, raw));
+}
+__device__ __forceinline__ float2 gate2(float2 w, int raw) {
+  return raw ? make_float2(gate_sig(w.x), gate_sig(w.y)) : w;
+}
+
+// The int8 form of one group (a warp's 64 channels) of a row.
+__device__ __forceinline__ void put_int8(float2 x, int8_t* codes, float* scale, int lane) {
+  const unsigned top = __reduce_max_sync(0xffffffffu, max(abs_bits(x.x), abs_bits(x.y)));
+  const GroupScale s = group_scale(top);
+  const int a = int8_code(x.x, s), b = int8_code(x.y, s);
+  *reinterpret_cast<short*>(codes) = (short)((a & 0xff) | (b << 8));
+  if (lane == 0) *scale = s.scale;
+}
+
+struct Args {
+  const void *v, *w, *g;
+  int8_t *v8, *w8;        // int8 checkpoints, or NULL
+  float *vs, *ws;         // their scales
+  const float *h0, *dout, *dhf;
+  float *o, *hf, *kept;
+  void *dv, *dw, *dg;
+  float* dh0;
+  int T, HD, tiles, raw;
+};
+
+template <typename T, bool SAVE8>
+__global__ void __launch_bounds__(256) k_recur_fwd(const Args p) {
+  __shared__ float4 map[kWarps][32];   // (a, b) of two channels
+  __shared__ float2 state[32];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int groups = p.HD / kGroup, bb = blockIdx.x / groups, cg = blockIdx.x % groups;
+  const int ch = cg * kGroup + 2 * lane;
+  const size_t row0 = (size_t)bb * p.T;
+  if (warp == 0)
+    state[lane] = p.h0 ? *reinterpret_cast<const float2*>(p.h0 + (size_t)bb * p.HD + ch)
+                       : make_float2(0.f, 0.f);
+  for (int tile = 0; tile < p.tiles; ++tile) {
+    const int t0 = tile * kTile + warp * kRows;
+    float2 a[kRows], x[kRows];
+    float4 m = make_float4(1.f, 0.f, 1.f, 0.f);
+#pragma unroll
+    for (int r = 0; r < kRows; ++r) {
+      a[r] = make_float2(1.f, 1.f);
+      x[r] = make_float2(0.f, 0.f);
+      if (t0 + r < p.T) {
+        const size_t at = (row0 + t0 + r) * p.HD + ch;
+        const float2 v = ld2(static_cast<const T*>(p.v) + at);
+        const float2 w = ld2(static_cast<const T*>(p.w) + at);
+        a[r] = decay2(ld2(static_cast<const T*>(p.g) + at), p.raw);
+        if constexpr (SAVE8) {
+          put_int8(v, p.v8 + at, p.vs + at / kGroup, lane);
+          put_int8(w, p.w8 + at, p.ws + at / kGroup, lane);
+        }
+        const float2 y = gate2(w, p.raw);
+        x[r] = make_float2(y.x * v.x, y.y * v.y);
+      }
+      m.x *= a[r].x; m.y = fmaf(a[r].x, m.y, x[r].x);
+      m.z *= a[r].y; m.w = fmaf(a[r].y, m.w, x[r].y);
+    }
+    map[warp][lane] = m;
+    __syncthreads();
+    float2 h = state[lane];
+    if (warp == 0 && p.kept)
+      *reinterpret_cast<float2*>(p.kept + ((size_t)bb * p.tiles + tile) * p.HD + ch) = h;
+    for (int j = 0; j < warp; ++j) {
+      const float4 z = map[j][lane];
+      h.x = fmaf(z.x, h.x, z.y);
+      h.y = fmaf(z.z, h.y, z.w);
+    }
+#pragma unroll
+    for (int r = 0; r < kRows; ++r) {
+      h.x = fmaf(a[r].x, h.x, x[r].x);
+      h.y = fmaf(a[r].y, h.y, x[r].y);
+      if (t0 + r < p.T) st2(p.o + (row0 + t0 + r) * p.HD + ch, h);
+      if (t0 + r == p.T - 1) *reinterpret_cast<float2*>(p.hf + (size_t)bb * p.HD + ch) = h;
+    }
+    __syncthreads();
+    if (warp == kWarps - 1) state[lane] = h;
+  }
+}
+
+template <typename T, bool FROM8>
+__global__ void __launch_bounds__(256) k_recur_bwd(const Args p) {
+  __shared__ float4 fmap[kWarps][32], rmap[kWarps][32];
+  __shared__ float2 carry[32];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int groups = p.HD / kGroup, bb = blockIdx.x / groups, cg = blockIdx.x % groups;
+  const int ch = cg * kGroup + 2 * lane;
+  const size_t row0 = (size_t)bb * p.T;
+  if (warp == 0)
+    carry[lane] = p.dhf ? *reinterpret_cast<const float2*>(p.dhf + (size_t)bb * p.HD + ch)
+                        : make_float2(0.f, 0.f);
+  for (int tile = p.tiles - 1; tile >= 0; --tile) {
+    const int t0 = tile * kTile + warp * kRows;
+    float2 a[kRows], v[kRows], w[kRows], d[kRows], sg[kRows];
+#pragma unroll
+    for (int r = 0; r < kRows; ++r) {
+      a[r] = make_float2(1.f, 1.f);
+      v[r] = w[r] = d[r] = sg[r] = make_float2(0.f, 0.f);
+      if (t0 + r < p.T) {
+        const size_t at = (row0 + t0 + r) * p.HD + ch;
+        if constexpr (FROM8) {
+          const float vs = p.vs[at / kGroup], ws = p.ws[at / kGroup];
+          v[r] = ld2(p.v8 + at);
+          w[r] = ld2(p.w8 + at);
+          v[r].x *= vs; v[r].y *= vs;
+          w[r].x *= ws; w[r].y *= ws;
+        } else {
+          v[r] = ld2(static_cast<const T*>(p.v) + at);
+          w[r] = ld2(static_cast<const T*>(p.w) + at);
+        }
+        sg[r] = ld2(static_cast<const T*>(p.g) + at);
+        a[r] = decay2(sg[r], p.raw);
+        w[r] = gate2(w[r], p.raw);
+        d[r] = ld2(p.dout + at);
+      }
+    }
+    float4 m = make_float4(1.f, 0.f, 1.f, 0.f), n = m;
+#pragma unroll
+    for (int r = 0; r < kRows; ++r) {
+      m.x *= a[r].x; m.y = fmaf(a[r].x, m.y, w[r].x * v[r].x);
+      m.z *= a[r].y; m.w = fmaf(a[r].y, m.w, w[r].y * v[r].y);
+    }
+#pragma unroll
+    for (int r = kRows - 1; r >= 0; --r) {
+      n.y = a[r].x * (d[r].x + n.y);
+      n.w = a[r].y * (d[r].y + n.w);
+    }
+    n.x = m.x;
+    n.z = m.z;
+    fmap[warp][lane] = m;
+    rmap[warp][lane] = n;
+    __syncthreads();
+    float2 h = *reinterpret_cast<const float2*>(p.kept + ((size_t)bb * p.tiles + tile) * p.HD + ch);
+    for (int j = 0; j < warp; ++j) {
+      const float4 z = fmap[j][lane];
+      h.x = fmaf(z.x, h.x, z.y);
+      h.y = fmaf(z.z, h.y, z.w);
+    }
+    float2 c = carry[lane];
+    for (int j = kWarps - 1; j > warp; --j) {
+      const float4 z = rmap[j][lane];
+      c.x = fmaf(z.x, c.x, z.y);
+      c.y = fmaf(z.z, c.y, z.w);
+    }
+    float2 before[kRows];
+#pragma unroll
+    for (int r = 0; r < kRows; ++r) {
+      before[r] = h;
+      h.x = fmaf(a[r].x, h.x, w[r].x * v[r].x);
+      h.y = fmaf(a[r].y, h.y, w[r].y * v[r].y);
+    }
+#pragma unroll
+    for (int r = kRows - 1; r >= 0; --r) {
+      const float2 dh = make_float2(d[r].x + c.x, d[r].y + c.y);
+      c = make_float2(a[r].x * dh.x, a[r].y * dh.y);
+      if (t0 + r < p.T) {
+        const size_t at = (row0 + t0 + r) * p.HD + ch;
+        float2 dw = make_float2(v[r].x * dh.x, v[r].y * dh.y);
+        float2 dg = make_float2(before[r].x * c.x, before[r].y * c.y);
+        if (p.raw) {
+          // d sigmoid(x) = w (1 - w); dg/dx = -sigmoid(x)
+          dw.x *= w[r].x * (1.f - w[r].x);
+          dw.y *= w[r].y * (1.f - w[r].y);
+          dg.x *= -sig_from(expf(-fabsf(sg[r].x)), sg[r].x > 0.f);
+          dg.y *= -sig_from(expf(-fabsf(sg[r].y)), sg[r].y > 0.f);
+        }
+        st2(static_cast<T*>(p.dv) + at, make_float2(w[r].x * dh.x, w[r].y * dh.y));
+        st2(static_cast<T*>(p.dw) + at, dw);
+        st2(static_cast<T*>(p.dg) + at, dg);
+      }
+    }
+    __syncthreads();
+    if (warp == 0) carry[lane] = c;
+    __syncthreads();
+  }
+  if (warp == 0)
+    *reinterpret_cast<float2*>(p.dh0 + (size_t)bb * p.HD + ch) = carry[lane];
+}
+
+int check(int dtype, int B, int T, int H, int D) {
+  if (dtype != GDN2_F32 && dtype != GDN2_BF16)
+    return report_error(GDN2_ERR_INVALID, "gdn2_recur: unsupported dtype code");
+  if (B <= 0 || T <= 0 || H <= 0)
+    return report_error(GDN2_ERR_INVALID, "gdn2_recur: empty problem B*T*H");
+  if (D != 64 && D != 128 && D != 256)
+    return report_error(GDN2_ERR_INVALID, "gdn2_recur: head dim D unsupported (64, 128 or 256)");
+  if (T > (1 << 30) || (long)H * D > (1 << 24) || (long)B * H * D / kGroup > 0x7fffffffL)
+    return report_error(GDN2_ERR_INVALID, "gdn2_recur: too many tokens or channels");
+  return GDN2_OK;
+}
+
+bool misaligned(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) != 0; }
+
+// The status header that gdn2_workspace_status() reads, cleared as by every
+// entry point that takes a workspace.
+int clear_status(void* workspace, cudaStream_t s) {
+  char* hdr = reinterpret_cast<char*>((reinterpret_cast<uintptr_t>(workspace) + 255) & ~(uintptr_t)255);
+  const cudaError_t e = cudaMemsetAsync(hdr, 0, 256, s);
+  return e == cudaSuccess ? GDN2_OK : report_error(GDN2_ERR_CUDA, cudaGetErrorString(e));
+}
+
+int launched() {
+  const cudaError_t e = cudaGetLastError();
+  return e == cudaSuccess ? GDN2_OK : report_error(GDN2_ERR_CUDA, cudaGetErrorString(e));
+}
+
+}  // namespace
+
+extern "C" size_t gdn2_recur_kept_floats(int B, int T, int H, int D) {
+  if (check(GDN2_F32, B, T, H, D)) return 0;
+  return (size_t)B * ((T + kTile - 1) / kTile) * H * D;
+}
+
+extern "C" size_t gdn2_recur_workspace_bytes(int B, int T, int H, int D) {
+  if (check(GDN2_F32, B, T, H, D)) return 0;
+  return 512;
+}
+
+extern "C" int gdn2_recur_fwd(int dtype, const void* v, const void* w, const void* g,
+                              const float* h0, float* o, float* h_final, float* kept, void* v8,
+                              float* v_scales, void* w8, float* w_scales, void* workspace,
+                              size_t workspace_bytes, int B, int T, int H, int D, void* stream) {
+  const int raw = (dtype & GDN2_GATES_RAW) != 0;
+  dtype &= ~GDN2_GATES_RAW;
+  const int rc = check(dtype, B, T, H, D);
+  if (rc) return rc;
+  const bool save8 = v8 || w8 || v_scales || w_scales;
+  if (!v || !w || !g || !o || !h_final || (save8 && (!v8 || !w8 || !v_scales || !w_scales)))
+    return report_error(GDN2_ERR_INVALID, "gdn2_recur_fwd: null buffer pointer");
+  if (misaligned(v) || misaligned(w) || misaligned(g) || misaligned(h0) || misaligned(o) ||
+      misaligned(h_final) || misaligned(kept) || misaligned(v8) || misaligned(w8))
+    return report_error(GDN2_ERR_INVALID, "gdn2_recur_fwd: buffers must be 16-byte aligned");
+  if (T > kTile && (!workspace || workspace_bytes < gdn2_recur_workspace_bytes(B, T, H, D)))
+    return report_error(GDN2_ERR_WORKSPACE, "gdn2_recur_fwd: workspace too small");
+  Args p{};
+  p.v = v; p.w = w; p.g = g; p.h0 = h0; p.o = o; p.hf = h_final; p.kept = kept;
+  p.v8 = static_cast<int8_t*>(v8); p.w8 = static_cast<int8_t*>(w8);
+  p.vs = v_scales; p.ws = w_scales;
+  p.T = T; p.HD = H * D; p.tiles = (T + kTile - 1) / kTile; p.raw = raw;
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  if (T > kTile) {
+    const int e = clear_status(workspace, s);
+    if (e) return e;
+  }
+  const unsigned grid = (unsigned)((size_t)B * H * D / kGroup);
+  if (dtype == GDN2_F32) {
+    if (save8) k_recur_fwd<float, true><<<grid, 256, 0, s>>>(p);
+    else k_recur_fwd<float, false><<<grid, 256, 0, s>>>(p);
+  } else {
+    if (save8) k_recur_fwd<__nv_bfloat16, true><<<grid, 256, 0, s>>>(p);
+    else k_recur_fwd<__nv_bfloat16, false><<<grid, 256, 0, s>>>(p);
+  }
+  return launched();
+}
+
+extern "C" int gdn2_recur_bwd(int dtype, const void* v, const void* w, const void* g,
+                              const void* v8, const float* v_scales, const void* w8,
+                              const float* w_scales, const float* kept, const float* dout,
+                              const float* dh_final, void* dv, void* dw, void* dg, float* dh0,
+                              void* workspace, size_t workspace_bytes, int B, int T, int H, int D,
+                              void* stream) {
+  const int raw = (dtype & GDN2_GATES_RAW) != 0;
+  dtype &= ~GDN2_GATES_RAW;
+  const int rc = check(dtype, B, T, H, D);
+  if (rc) return rc;
+  const bool from8 = v8 || w8 || v_scales || w_scales;
+  if (from8 ? (!v8 || !w8 || !v_scales || !w_scales) : (!v || !w))
+    return report_error(GDN2_ERR_INVALID, "gdn2_recur_bwd: null buffer pointer");
+  if (!g || !kept || !dout || !dv || !dw || !dg || !dh0)
+    return report_error(GDN2_ERR_INVALID, "gdn2_recur_bwd: null buffer pointer");
+  if (misaligned(v) || misaligned(w) || misaligned(g) || misaligned(v8) || misaligned(w8) ||
+      misaligned(kept) || misaligned(dout) || misaligned(dh_final) || misaligned(dv) ||
+      misaligned(dw) || misaligned(dg) || misaligned(dh0))
+    return report_error(GDN2_ERR_INVALID, "gdn2_recur_bwd: buffers must be 16-byte aligned");
+  if (T > kTile && (!workspace || workspace_bytes < gdn2_recur_workspace_bytes(B, T, H, D)))
+    return report_error(GDN2_ERR_WORKSPACE, "gdn2_recur_bwd: workspace too small");
+  Args p{};
+  p.v = v; p.w = w; p.g = g;
+  p.v8 = static_cast<int8_t*>(const_cast<void*>(v8));
+  p.w8 = static_cast<int8_t*>(const_cast<void*>(w8));
+  p.vs = const_cast<float*>(v_scales); p.ws = const_cast<float*>(w_scales);
+  p.kept = const_cast<float*>(kept); p.dout = dout; p.dhf = dh_final;
+  p.dv = dv; p.dw = dw; p.dg = dg; p.dh0 = dh0;
+  p.T = T; p.HD = H * D; p.tiles = (T + kTile - 1) / kTile; p.raw = raw;
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  if (T > kTile) {
+    const int e = clear_status(workspace, s);
+    if (e) return e;
+  }
+  const unsigned grid = (unsigned)((size_t)B * H * D / kGroup);
+  if (dtype == GDN2_F32) {
+    if (from8) k_recur_bwd<float, true><<<grid, 256, 0, s>>>(p);
+    else k_recur_bwd<float, false><<<grid, 256, 0, s>>>(p);
+  } else {
+    if (from8) k_recur_bwd<__nv_bfloat16, true><<<grid, 256, 0, s>>>(p);
+    else k_recur_bwd<__nv_bfloat16, false><<<grid, 256, 0, s>>>(p);
+  }
+  return launched();
+}

@@ -15,3 +15,10 @@ from . import sequence_parallel  # noqa: E402,F401
 from .gdn2_decode import gdn2_decode  # noqa: E402,F401
 from .streaming import gdn2_fwd_bwd  # noqa: E402,F401
 from .segmented import gdn2_segmented_forward_trainable  # noqa: E402,F401
+from .gdn2_checkpoint import (  # noqa: E402,F401
+    Gdn2Checkpoint, gdn2_checkpoint_pack, gdn2_checkpoint_unpack)
+from .gdn2_state_cache import (  # noqa: E402,F401
+    Gdn2StateCache, gdn2_decode_cached, gdn2_state_read, gdn2_state_write)
+from .gdn2_recurrence import (  # noqa: E402,F401
+    gdn2_linear_recurrence, gdn2_linear_recurrence_backward, gdn2_linear_recurrence_trainable,
+    gdn2_linear_recurrence_with_residuals)

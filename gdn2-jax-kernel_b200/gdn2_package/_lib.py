@@ -55,6 +55,15 @@ SIGNATURES = {
     "gdn2_stage_wy_dqkg": (_i, [_vp] * 20 + [_i] * 3 + [_f, _f, _vp]),
     "gdn2_stage_intra_bwd": (_i, [_i] + [_vp] * 11 + [_i] * 6 + [_f, _f, _vp]),
     "gdn2_stage_revcumsum": (_i, [_vp, _vp, _i, _i, _i, _f, _vp]),
+    "gdn2_int8_pack": (_i, [_i, _i, _vp, _vp, _vp, _sz, _vp]),
+    "gdn2_int8_unpack": (_i, [_i, _i, _vp, _vp, _vp, _sz, _vp]),
+    "gdn2_state_write": (_i, [_vp] * 4 + [_i] * 4 + [_f, _vp]),
+    "gdn2_state_read": (_i, [_i] + [_vp] * 4 + [_i] * 4 + [_vp]),
+    "gdn2_decode_cached": (_i, [_i] + [_vp] * 11 + [_i] * 5 + [_f, _f, _vp]),
+    "gdn2_recur_kept_floats": (_sz, [_i] * 4),
+    "gdn2_recur_workspace_bytes": (_sz, [_i] * 4),
+    "gdn2_recur_fwd": (_i, [_i] + [_vp] * 12 + [_sz] + [_i] * 4 + [_vp]),
+    "gdn2_recur_bwd": (_i, [_i] + [_vp] * 15 + [_sz] + [_i] * 4 + [_vp]),
     "gdn2_diag_read": (_i, [_vp, _sz, _vp, _i, ctypes.POINTER(ctypes.c_int),
                             ctypes.POINTER(ctypes.c_float)]),
 }

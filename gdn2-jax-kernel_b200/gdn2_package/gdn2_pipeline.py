@@ -17,6 +17,7 @@ import torch
 
 from . import gdn2_bwd as _bwd
 from . import gdn2_fwd as _fwd
+from .gdn2_checkpoint import Gdn2Checkpoint, gdn2_checkpoint_pack, gdn2_checkpoint_unpack
 
 _FINAL_CLIP = 1e4  # gdn2_pipeline.py:34
 
@@ -61,15 +62,48 @@ class _Gdn2Core(torch.autograd.Function):
         return dq, dk, dv, dw, db, dg, dh0, None, None
 
 
-def gdn2_pallas_forward_trainable(q, k, v, w, b, g, scale, h0=None, recompute=False):
+class _Gdn2CoreInt8(torch.autograd.Function):
+    """_Gdn2Core that keeps q, k, v, w, b in 8 bits and recomputes the forward
+    from the restored values in the backward."""
+
+    @staticmethod
+    def forward(ctx, q, k, v, w, b, g, h0, scale):
+        o, h_final = _fwd.gdn2_pallas_forward(q, k, v, w, b, g, scale, h0)
+        kept = gdn2_checkpoint_pack(q, k, v, w, b)
+        ctx.scale, ctx.dtypes, ctx.on_host = scale, kept.dtypes, kept.on_host
+        ctx.save_for_backward(g, h0, *kept.codes, *kept.scales)
+        return o, h_final
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, do, dh_final):
+        g, h0, *kept = ctx.saved_tensors
+        if do is None:
+            do = torch.zeros(g.shape, dtype=torch.float32, device=g.device)
+        q, k, v, w, b = gdn2_checkpoint_unpack(
+            Gdn2Checkpoint(kept[:5], kept[5:], ctx.dtypes, ctx.on_host))
+        grads = _bwd.gdn2_backward(q, k, v, w, b, g, ctx.scale, h0, do, dh_final)
+        return *grads, None
+
+
+def gdn2_pallas_forward_trainable(q, k, v, w, b, g, scale, h0=None, recompute=False,
+                                  checkpoint=None):
     """Trainable Gated DeltaNet-2 forward with the fused backward.
 
     Args: q, k, v, w, b, g (batch, seq_len, heads, d_head) CUDA tensors;
     scale a Python float; h0 (batch, heads, d_head, d_head), zero if None.
     Returns out (batch, seq_len, heads, d_head) and h_final
     (batch, heads, d_head, d_head), both float32.
+
+    checkpoint="int8" keeps q, k, v, w, b in 8 bits (gdn2_checkpoint_pack) and
+    g, h0 as they are, and recomputes the forward: the gradients are those at
+    the restored inputs, the outputs those of the inputs.
     """
+    if checkpoint not in (None, "int8"):
+        raise _fwd.Gdn2ShapeError(f"checkpoint={checkpoint!r}: None or 'int8'")
     B, T, H, D = q.shape
     if h0 is None:
         h0 = torch.zeros((B, H, D, D), dtype=torch.float32, device=q.device)
+    if checkpoint == "int8":
+        return _Gdn2CoreInt8.apply(q, k, v, w, b, g, h0, float(scale))
     return _Gdn2Core.apply(q, k, v, w, b, g, h0, float(scale), bool(recompute))

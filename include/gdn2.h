@@ -33,7 +33,7 @@ extern "C" {
 
 enum { GDN2_F32 = 0, GDN2_BF16 = 1 };
 /* OR-ed into the dtype argument of gdn2_fwd / gdn2_bwd / gdn2_fwd_noalloc /
- * gdn2_decode: w, b, g are pre-activations and the kernels apply
+ * gdn2_decode / gdn2_decode_cached / gdn2_recur_fwd / gdn2_recur_bwd: w, b, g are pre-activations and the kernels apply
  * w = sigmoid(w), b = sigmoid(b), g = -softplus(g) as they load them (the
  * activations the reference leaves to its caller, README.md:60-68).
  * gdn2_bwd then returns dw, db, dg with respect to the pre-activations.  The
@@ -243,6 +243,83 @@ int gdn2_stage_revcumsum(const float* dgc, float* dg, int n_chunks, int BT, int 
 int gdn2_decode(int dtype, const void* q, const void* k, const void* v, const void* w,
                 const void* b, const void* g, const float* h0, float* o, float* h_final, int B,
                 int T, int H, int D, float scale, float clip, void* stream);
+
+/* The int8 form of values (activation checkpoints, cached states): groups of
+ * 64 consecutive values share one float32 scale; code = rint(127 x / max|x|)
+ * with ties to even, decided exactly, scale = max|x| / 127, value = code *
+ * scale (off by at most max|x| / 254).  A group whose largest |x| is below
+ * 2^-100 is stored as zeros; one that holds a NaN or an infinity gets a NaN
+ * scale and reads back as NaN throughout.  Values and codes are 16-byte
+ * aligned.  No counterpart in the reference.
+ *
+ * Pack / unpack n_tensors tensors (1 .. GDN2_INT8_MAX_TENSORS) of n values each
+ * (a multiple of 64) in one launch: values[i] of `dtype`, codes[i] n int8,
+ * scales[i] n / 64 float32.  The pointer arrays are host arrays, read before
+ * the call returns. */
+#define GDN2_INT8_MAX_TENSORS 8
+int gdn2_int8_pack(int dtype, int n_tensors, const void* const* values, void* const* codes,
+                   float* const* scales, size_t n, void* stream);
+int gdn2_int8_unpack(int dtype, int n_tensors, void* const* values, const void* const* codes,
+                     const float* const* scales, size_t n, void* stream);
+
+/* int8 cache of recurrent states: codes (S, H, D, D) int8 and scales
+ * (S, H, D, D / 64) float32 hold one state per slot.  Row b of a call uses slot
+ * slots[b] (int32, device; NULL: slot b, with B <= S); D is 64, 128 or 256.
+ *   write: h (B, H, D, D) float32, through the CLIP sanitiser like the states
+ *          of gdn2_decode.  A slot outside the cache (-1 by convention) drops
+ *          the row; of several rows that name one slot the last is kept.
+ *   read:  h (B, H, D, D) of `dtype`.  A slot of -1 reads as the zero state,
+ *          any other slot outside the cache as NaN. */
+int gdn2_state_write(const float* h, const int* slots, void* codes, float* scales, int B, int S,
+                     int H, int D, float clip, void* stream);
+int gdn2_state_read(int dtype, const void* codes, const float* scales, const int* slots, void* h,
+                    int B, int S, int H, int D, void* stream);
+
+/* gdn2_decode on that cache: row b starts from slot src[b] (-1: the zero
+ * state), runs T tokens with the state in float32 and stores it in slot dst[b]
+ * (-1: dropped).  src = dst updates the rows in place; several rows may start
+ * from one slot (a shared prefix).  src and dst both NULL: slot b.  A row whose
+ * slots lie outside the cache, or whose destination is another row's source or
+ * destination, gets NaN outputs and stores nothing: its result would depend on
+ * the order of blocks.  D is 64 or 128. */
+int gdn2_decode_cached(int dtype, const void* q, const void* k, const void* v, const void* w,
+                       const void* b, const void* g, void* codes, float* scales, const int* src,
+                       const int* dst, float* o, int B, int T, int H, int D, int S, float scale,
+                       float clip, void* stream);
+
+/* Gated linear recurrence per channel (no counterpart in the reference):
+ *   h_t = e^{g_t} h_{t-1} + w_t v_t,  o_t = h_t
+ * on v, w, g (B, T, H, D) of `dtype` (GDN2_GATES_RAW as above), states
+ * (B, H, D) float32, o float32; any T >= 1, D 64, 128 or 256, no sanitiser.
+ * g may be -inf (the state restarts).  Buffers are 16-byte aligned.
+ *
+ * gdn2_recur_fwd: h0 may be NULL (zero).  `kept` (NULL: none) receives the
+ * gdn2_recur_kept_floats() floats that the backward needs: the state before
+ * every GDN2_RECUR_INTERVAL-th token, (B, ceil(T / 64), H, D).  v8, v_scales,
+ * w8, w_scales (all or none) receive v and w (as given, before any activation)
+ * in the int8 form.
+ *
+ * gdn2_recur_bwd: with v8 .. w_scales NULL the gradients are those of the
+ * forward; with them (v and w may then be NULL) those at the restored values,
+ * whose states restart from the kept ones every GDN2_RECUR_INTERVAL tokens.
+ * dout float32, dh_final float32 (NULL: zero); dv, dw, dg of `dtype`, dh0
+ * float32.
+ *
+ * workspace: gdn2_recur_workspace_bytes(), scratch of one call (its status is
+ * read with gdn2_workspace_status); none is needed for T up to
+ * GDN2_RECUR_INTERVAL. */
+#define GDN2_RECUR_INTERVAL 64
+size_t gdn2_recur_kept_floats(int B, int T, int H, int D);
+size_t gdn2_recur_workspace_bytes(int B, int T, int H, int D);
+int gdn2_recur_fwd(int dtype, const void* v, const void* w, const void* g, const float* h0,
+                   float* o, float* h_final, float* kept, void* v8, float* v_scales, void* w8,
+                   float* w_scales, void* workspace, size_t workspace_bytes, int B, int T, int H,
+                   int D, void* stream);
+int gdn2_recur_bwd(int dtype, const void* v, const void* w, const void* g, const void* v8,
+                   const float* v_scales, const void* w8, const float* w_scales, const float* kept,
+                   const float* dout, const float* dh_final, void* dv, void* dw, void* dg,
+                   float* dh0, void* workspace, size_t workspace_bytes, int B, int T, int H, int D,
+                   void* stream);
 
 /* Per-launch device timing (test and benchmark support; no counterpart in the
  * reference).  When enabled, every kernel launch of gdn2_fwd / gdn2_bwd is

@@ -1,0 +1,269 @@
+"""The gated linear recurrence: both directions against a float64 token loop,
+the int8 checkpoints, autograd, differences, CUDA graphs and streams."""
+import pytest
+import torch
+
+from conftest import cuda_ok
+
+pytestmark = [pytest.mark.gpu, pytest.mark.skipif(not cuda_ok(), reason="needs a CUDA device")]
+
+from int8_ref import assert_close, linrec64, values64  # noqa: E402
+from gdn2_package import (gdn2_fwd, gdn2_linear_recurrence,  # noqa: E402
+                          gdn2_linear_recurrence_backward, gdn2_linear_recurrence_trainable,
+                          gdn2_linear_recurrence_with_residuals)
+
+GRADS = ("dv", "dw", "dg", "dh0")
+
+
+@pytest.fixture(autouse=True)
+def _gates():
+    saved = gdn2_fwd.GATES
+    yield
+    gdn2_fwd.GATES = saved
+
+
+def make(B, T, H, D, dtype=torch.float32, seed=0, raw=False, h0=True, g_shift=-3.0):
+    gen = torch.Generator(device="cuda").manual_seed(seed)
+    nrm = lambda *s: torch.randn(s, generator=gen, device="cuda")  # noqa: E731
+    x = dict(v=nrm(B, T, H, D), w=nrm(B, T, H, D), g=1.5 * nrm(B, T, H, D) + g_shift)
+    if not raw:
+        x["w"] = torch.sigmoid(x["w"])
+        x["g"] = -torch.nn.functional.softplus(x["g"])
+    x = {n: t.to(dtype) for n, t in x.items()}
+    x["h0"] = nrm(B, H, D) if h0 else None
+    return x, nrm(B, T, H, D), nrm(B, H, D)
+
+
+def check(x, do, dh, int8=False, raw=False):
+    o, h, res = gdn2_linear_recurrence_with_residuals(**x, checkpoint="int8" if int8 else None)
+    grads = gdn2_linear_recurrence_backward(res, do, dh)
+    v8, w8 = (values64(x["v"]), values64(x["w"])) if int8 else (None, None)
+    want = linrec64(x["v"], x["w"], x["g"], x["h0"], do, dh, v8, w8, raw)
+    assert o.dtype == h.dtype == grads[3].dtype == torch.float32
+    assert_close(o, *want["o"], "o")
+    assert_close(h, *want["h"], "h")
+    assert torch.equal(h, o[:, -1])
+    for name, got in zip(GRADS, grads):
+        assert_close(got, *want[name], name)
+        assert name == "dh0" or got.dtype == x["v"].dtype
+
+
+@pytest.mark.parametrize("B,T,H,D", [(1, 1, 1, 64), (3, 1, 5, 128), (2, 7, 3, 64), (1, 63, 1, 256),
+                                     (2, 64, 3, 128), (1, 65, 1, 64), (5, 200, 3, 64),
+                                     (1, 513, 3, 128), (2, 1029, 1, 64), (1, 4099, 2, 128)])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("int8", [False, True])
+def test_both_directions(B, T, H, D, dtype, int8):
+    x, do, dh = make(B, T, H, D, dtype, seed=T + H)
+    check(x, do, dh, int8)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("int8", [False, True])
+def test_raw_gates(dtype, int8):
+    gdn2_fwd.GATES = "raw"
+    x, do, dh = make(2, 150, 3, 64, dtype, seed=5, raw=True)
+    check(x, do, dh, int8, raw=True)
+
+
+def test_raw_gates_at_their_ends():
+    """Pre-activations far out on both sides: e^g of 1 and of 0, w of 0 and 1."""
+    gdn2_fwd.GATES = "raw"
+    x, do, dh = make(1, 96, 1, 64, seed=6, raw=True)
+    far = torch.tensor([-float("inf"), -200.0, -30.0, 30.0, 90.0, 200.0], device="cuda")
+    x["g"].view(-1)[:6 * 64] = far.repeat_interleave(64)
+    x["w"].view(-1)[64 * 6:64 * 12] = far.clamp(-80, 80).repeat_interleave(64)
+    check(x, do, dh, raw=True)
+
+
+@pytest.mark.parametrize("T", [40, 64, 300])
+def test_restarts_and_fast_and_slow_decay(T):
+    """g of -inf restarts the state; g of 0 keeps it; g of -1e4 is a restart too."""
+    x, do, dh = make(2, T, 2, 64, seed=7)
+    x["g"][:, T // 3] = -float("inf")
+    x["g"][:, T // 2, 0] = -1e4
+    x["g"][0, :, 1] = 0.0
+    check(x, do, dh)
+    o, _ = gdn2_linear_recurrence(**x)
+    fresh = torch.isinf(x["g"])
+    assert fresh.any() and torch.equal(o[fresh], (x["w"] * x["v"])[fresh])
+
+
+def test_padded_tokens_leave_the_state():
+    """Zero tokens (v = w = g = 0) behind a sequence change nothing before them
+    and keep the state.  Its bits may differ: on the way through the padded
+    tiles it is formed from joined maps, whose 2 roundings a join the bound of
+    linrec64 counts."""
+    x, do, dh = make(2, 130, 2, 128, seed=8)
+    for n in ("v", "w", "g"):
+        x[n][1, 77:] = 0
+    o, h = gdn2_linear_recurrence(**x)
+    short = {n: t[1:, :77] if n != "h0" else t[1:] for n, t in x.items()}
+    o1, h1 = gdn2_linear_recurrence(**short)
+    assert torch.equal(o[1:, :77], o1)
+    want = linrec64(short["v"], short["w"], short["g"], short["h0"])
+    assert_close(h1, *want["h"], "h")
+    assert_close(h[1:], *want["h"], "h of the padded row")
+
+
+def test_no_state_no_final_gradient_and_segments():
+    """h0 and dh_final may be missing; a sequence in two calls is the sequence."""
+    x, do, _ = make(2, 200, 3, 64, seed=9, h0=False)
+    check(x, do, None)
+    o, h = gdn2_linear_recurrence(**x)
+    a = {n: t[:, :90] for n, t in x.items() if n != "h0"}
+    b = {n: t[:, 90:] for n, t in x.items() if n != "h0"}
+    oa, ha = gdn2_linear_recurrence(**a)
+    ob, hb = gdn2_linear_recurrence(**b, h0=ha)
+    want = linrec64(x["v"], x["w"], x["g"], None)
+    assert_close(torch.cat([oa, ob], 1), *want["o"], "o")
+    assert_close(hb, *want["h"], "h")
+
+
+@pytest.mark.parametrize("int8", [None, "int8"])
+def test_autograd_is_the_backward(int8):
+    x, do, dh = make(2, 150, 2, 64, seed=10)
+    o, h, res = gdn2_linear_recurrence_with_residuals(**x, checkpoint=int8)
+    want = gdn2_linear_recurrence_backward(res, do, dh)
+    leaves = [t.clone().requires_grad_(True) for t in x.values()]
+    o2, h2 = gdn2_linear_recurrence_trainable(*leaves, checkpoint=int8)
+    got = torch.autograd.grad((o2, h2), leaves, (do, dh))
+    assert torch.equal(o, o2) and torch.equal(h, h2)
+    for a, b in zip(got, want):
+        assert torch.equal(a, b)
+    # one output used, one leaf wanted, no h0
+    o3, _ = gdn2_linear_recurrence_trainable(leaves[0], x["w"], x["g"], checkpoint=int8)
+    (dv,) = torch.autograd.grad(o3, leaves[0], do)
+    _, _, res = gdn2_linear_recurrence_with_residuals(x["v"], x["w"], x["g"], checkpoint=int8)
+    assert torch.equal(dv, gdn2_linear_recurrence_backward(res, do)[0])
+    _, h4 = gdn2_linear_recurrence_trainable(*leaves, checkpoint=int8)
+    (dh0,) = torch.autograd.grad(h4, leaves[3], dh)
+    assert torch.isfinite(dh0).all()
+
+
+def test_a_changed_input_is_noticed():
+    x, do, dh = make(1, 70, 1, 64, seed=11)
+    leaves = [t.clone().requires_grad_(True) for t in x.values()]
+    o, h = gdn2_linear_recurrence_trainable(*leaves)
+    with torch.no_grad():
+        leaves[2].mul_(2)
+    with pytest.raises(RuntimeError, match="modified by an inplace"):
+        torch.autograd.grad(o, leaves[0], do)
+
+
+def test_gradients_against_differences():
+    """Central differences of sum(o do) + sum(h dh) in float64 on the values the
+    kernel saw, with the truncation error of step e bounded by e^2 times the
+    third derivative (v, w, h0 enter linearly; g through exponentials below 1)."""
+    x, do, dh = make(1, 70, 1, 64, seed=12)
+    _, _, res = gdn2_linear_recurrence_with_residuals(**x)
+    grads = gdn2_linear_recurrence_backward(res, do, dh)
+
+    def loss(x):
+        r = linrec64(x["v"], x["w"], x["g"], x["h0"])
+        return (r["o"][0] * do.double()).sum((0, 1, 2)) + (r["h"][0] * dh.double()).sum((0, 1))
+
+    e = 1e-4
+    for name, got in zip(("v", "w", "g", "h0"), grads):
+        for t in (0, 5, 63, 64, 69):
+            up, dn = ({n: a.double().clone() for n, a in x.items()} for _ in range(2))
+            at = (0, 0) if name == "h0" else (0, t, 0)
+            up[name][at] += e
+            dn[name][at] -= e
+            want = (loss(up) - loss(dn)) / (2 * e)   # per channel: channels do not mix
+            assert torch.allclose(got[at].double(), want, rtol=1e-4, atol=1e-4), (name, t)
+            if name == "h0":
+                break
+
+
+def test_strided_mixed_and_host_inputs():
+    x, do, dh = make(2, 90, 2, 64, seed=13)
+    o, h = gdn2_linear_recurrence(**x)
+    wide = torch.randn(2, 90, 2, 3 * 64, device="cuda")
+    wide[..., 64:128] = x["v"]
+    o2, _ = gdn2_linear_recurrence(wide[..., 64:128], x["w"].transpose(1, 2).contiguous().transpose(1, 2),
+                                   x["g"], x["h0"])
+    assert torch.equal(o, o2)
+    flat = torch.empty(x["v"].numel() + 1, device="cuda")
+    odd = flat[1:].view(x["v"].shape).copy_(x["v"])   # 4 bytes off a 16-byte boundary
+    assert torch.equal(o, gdn2_linear_recurrence(odd, x["w"], x["g"], x["h0"])[0])
+    oc, hc = gdn2_linear_recurrence(*[t.cpu() for t in x.values()])
+    assert oc.device.type == "cpu" and torch.equal(oc, o.cpu()) and torch.equal(hc, h.cpu())
+    # one float32 input makes the call float32; each gradient has its input's type
+    vb = x["v"].to(torch.bfloat16)
+    om, _, res = gdn2_linear_recurrence_with_residuals(vb, x["w"], x["g"], x["h0"])
+    assert torch.equal(om, gdn2_linear_recurrence(vb.float(), x["w"], x["g"], x["h0"])[0])
+    gm = gdn2_linear_recurrence_backward(res, do, dh)
+    assert gm[0].dtype == torch.bfloat16 and gm[1].dtype == torch.float32
+
+
+def test_same_answer_every_time_and_on_another_stream():
+    x, do, dh = make(4, 3000, 3, 128, seed=14)
+
+    def step():
+        o, h, res = gdn2_linear_recurrence_with_residuals(**x, checkpoint="int8")
+        return (o, h, *gdn2_linear_recurrence_backward(res, do, dh))
+
+    first = step()
+    for _ in range(5):
+        assert all(torch.equal(a, b) for a, b in zip(first, step()))
+    torch.cuda.synchronize()
+    side, other = torch.cuda.Stream(), torch.cuda.Stream()
+    with torch.cuda.stream(side):   # two calls at once
+        got = step()
+    with torch.cuda.stream(other):
+        more = step()
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) and torch.equal(a, c) for a, b, c in zip(first, got, more))
+
+
+@pytest.mark.parametrize("T", [1, 60, 700])
+def test_captured_and_replayed(T):
+    x, do, dh = make(2, T, 2, 64, seed=15)
+
+    def step():
+        o, h, res = gdn2_linear_recurrence_with_residuals(**x)
+        return (o, h, *gdn2_linear_recurrence_backward(res, do, dh))
+
+    step()
+    torch.cuda.synchronize()
+    graphs = []
+    pool = torch.cuda.graph_pool_handle()
+    for _ in range(2):   # two graphs on one pool: the second reuses the first's scratch
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, pool=pool):
+            out = step()
+        graphs.append((g, out))
+    y, _, _ = make(2, T, 2, 64, seed=16)
+    for n in x:
+        x[n].copy_(y[n])
+    want = step()
+    for g, out in graphs * 2:
+        for o in out:
+            o.fill_(float("nan"))
+        g.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(want, out))
+
+
+def test_long_sequence_of_slow_decay():
+    """131072 tokens of one head, decays near 1: the joins over 2048 tiles."""
+    x, do, dh = make(1, 131072, 1, 64, seed=17, g_shift=-7.0)
+    o, h, res = gdn2_linear_recurrence_with_residuals(**x)
+    dv, _, _, dh0 = gdn2_linear_recurrence_backward(res, do, dh)
+    a, put = torch.exp(x["g"].double()), (x["w"].double() * x["v"].double())
+    want = torch.empty_like(put)
+    s = x["h0"].double()
+    for t in range(131072):
+        s = torch.addcmul(put[:, t], a[:, t], s, out=want[:, t])
+    # terms k tokens back are off by 32 (k + 1) U and weigh a^k: about 32 U / (1 - a) of the sum
+    rel = float((o.double() - want).norm() / want.norm())
+    assert rel < 1e-5, rel
+    c = dh.double()
+    for t in range(131071, -1, -1):
+        d = do[:, t].double() + c
+        put[:, t] = x["w"][:, t].double() * d
+        c = a[:, t] * d
+    rel = float((dv.double() - put).norm() / put.norm())
+    assert rel < 1e-5, rel
+    assert torch.allclose(dh0.double(), c, rtol=1e-4, atol=1e-5)
