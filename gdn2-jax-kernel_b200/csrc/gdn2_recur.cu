@@ -16,6 +16,17 @@
 // it: every global byte moves once.  What moves bounds the kernels: float32
 // 16 bytes a value forward, 28 backward.
 //
+// The tiles of a sequence run at the same time.  Each publishes its map before
+// it waits for anything; sixteen tiles in a row form a group, and a tile walks
+// from the state that enters its group through the maps of the tiles before it
+// there.  The last tile of a group publishes the state that enters the next.
+// So a sequence of n tiles is n / 16 dependent steps, every state is formed by
+// the same operations whatever ran first (results do not depend on timing),
+// and a tile reads at most 16 published maps of 512 bytes.  Tiles are taken in
+// the order of time by a counter, so what a tile waits for has always started.
+// A published word is 64 bits, (a, b) of one channel, with the sign bit of a
+// (never negative) set: zeroed memory is "not yet", and no fence is needed.
+//
 // The forward keeps the state that enters each tile (1/64 of o).  The backward
 // rebuilds the states inside a tile from it, so it does not read o; with int8
 // checkpoints it does so from the 8-bit v and w, which makes its gradients
@@ -76,6 +87,59 @@ __device__ __forceinline__ void put_int8(float2 x, int8_t* codes, float* scale, 
   if (lane == 0) *scale = s.scale;
 }
 
+constexpr int kGroupTiles = 16;
+constexpr int kPolls = 1 << 22;   // about two seconds, then the status word is set
+
+// Scratch of one call with more than one tile, zeroed before the kernel.
+struct Scratch {
+  int* status;       // the header: [0] a wait ran out, [8] the tile counter
+  ulonglong2* maps;  // [tile][chain][32 lanes]: the maps of two channels
+  ulonglong2* enter; // [group][chain][32 lanes]: the states that enter groups 1..
+};
+size_t scratch_bytes(size_t tiles, size_t chains) {
+  return 512 + (tiles + tiles / kGroupTiles + 1) * chains * 512;
+}
+
+__device__ __forceinline__ unsigned long long word(float a, float b) {
+  return ((unsigned long long)__float_as_uint(b) << 32) | (__float_as_uint(a) | 0x80000000u);
+}
+__device__ __forceinline__ void publish(ulonglong2* p, float4 m) {
+  asm volatile("st.relaxed.gpu.global.v2.u64 [%0], {%1, %2};"
+               ::"l"(p), "l"(word(m.x, m.y)), "l"(word(m.z, m.w)) : "memory");
+}
+__device__ __forceinline__ ulonglong2 peek(const ulonglong2* p) {
+  ulonglong2 v;
+  asm volatile("ld.relaxed.gpu.global.v2.u64 {%0, %1}, [%2];" : "=l"(v.x), "=l"(v.y) : "l"(p) : "memory");
+  return v;
+}
+__device__ __forceinline__ bool there(ulonglong2 v) { return ((unsigned)v.x & (unsigned)v.y) >> 31; }
+__device__ __forceinline__ float4 unword(ulonglong2 v) {
+  return make_float4(__uint_as_float((unsigned)v.x & 0x7fffffffu), __uint_as_float((unsigned)(v.x >> 32)),
+                     __uint_as_float((unsigned)v.y & 0x7fffffffu), __uint_as_float((unsigned)(v.y >> 32)));
+}
+// Waits until the words at p are there in every lane, kPolls times at most; a
+// wait that runs out, here or elsewhere in the call, is in the status word and
+// ends this one too.
+__device__ float4 await(const ulonglong2* p, int* status) {
+  ulonglong2 v = peek(p);
+  for (int i = 1; !__all_sync(0xffffffffu, there(v)); ++i) {
+    if (i >= kPolls || (i % 4096 == 0 && *(volatile int*)status)) {
+      if ((threadIdx.x & 31) == 0) atomicExch(status, 1);
+      break;
+    }
+    v = peek(p);
+  }
+  return unword(v);
+}
+
+// m2 after m1, on two channels.
+__device__ __forceinline__ float4 after(float4 m2, float4 m1) {
+  return make_float4(m2.x * m1.x, fmaf(m2.x, m1.y, m2.y), m2.z * m1.z, fmaf(m2.z, m1.w, m2.w));
+}
+__device__ __forceinline__ float2 apply(float4 m, float2 h) {
+  return make_float2(fmaf(m.x, h.x, m.y), fmaf(m.z, h.y, m.w));
+}
+
 struct Args {
   const void *v, *w, *g;
   int8_t *v8, *w8;        // int8 checkpoints, or NULL
@@ -84,162 +148,191 @@ struct Args {
   float *o, *hf, *kept;
   void *dv, *dw, *dg;
   float* dh0;
-  int T, HD, tiles, raw;
+  Scratch s;
+  int T, HD, tiles, chains, raw;
 };
+
+// The tile of this CTA: (chain, index k in the order of the scan).
+struct Place { int chain, k; };
+__device__ __forceinline__ Place take_tile(const Args& p) {
+  __shared__ int ticket;
+  unsigned t = blockIdx.x;
+  if (p.tiles > 1) {
+    if (threadIdx.x == 0) ticket = atomicAdd(p.s.status + 8, 1);
+    __syncthreads();
+    t = (unsigned)ticket;
+  }
+  return {(int)(t % p.chains), (int)(t / p.chains)};
+}
+
+// The state that enters tile k of a chain, from the maps of its warps in the
+// order of the scan (map, complete: the caller has synchronised) and `first`,
+// the state that enters the sequence.
+struct Joint {
+  float4 mates[kGroupTiles][32];
+  float2 enter[32];
+};
+__device__ __forceinline__ float2 enter_tile(const Args& p, const Place at,
+                                             const float4 (*map)[32], Joint& joint,
+                                             const float* first) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int mate = at.k % kGroupTiles, group = at.k / kGroupTiles;
+  const bool last = at.k + 1 == p.tiles;
+  if (warp == 0 && !last && mate != kGroupTiles - 1) {
+    float4 m = map[0][lane];
+#pragma unroll
+    for (int j = 1; j < kWarps; ++j) m = after(map[j][lane], m);
+    publish(p.s.maps + ((size_t)at.k * p.chains + at.chain) * 32 + lane, m);
+  }
+  for (int i = warp; i < mate; i += kWarps)
+    joint.mates[i][lane] =
+        await(p.s.maps + ((size_t)(at.k - mate + i) * p.chains + at.chain) * 32 + lane, p.s.status);
+  if (warp == kWarps - 1) {
+    float2 h = make_float2(0.f, 0.f);
+    if (group) {
+      const float4 m = await(p.s.enter + ((size_t)group * p.chains + at.chain) * 32 + lane, p.s.status);
+      h = make_float2(m.y, m.w);
+    } else if (first) {
+      h = *reinterpret_cast<const float2*>(first + (size_t)at.chain * kGroup + 2 * lane);
+    }
+    joint.enter[lane] = h;
+  }
+  __syncthreads();
+  float2 h = joint.enter[lane];
+  for (int i = 0; i < mate; ++i) h = apply(joint.mates[i][lane], h);
+  if (warp == 0 && !last && mate == kGroupTiles - 1) {
+    float2 e = h;
+#pragma unroll
+    for (int j = 0; j < kWarps; ++j) e = apply(map[j][lane], e);
+    publish(p.s.enter + ((size_t)(group + 1) * p.chains + at.chain) * 32 + lane,
+            make_float4(0.f, e.x, 0.f, e.y));
+  }
+  return h;
+}
 
 template <typename T, bool SAVE8>
 __global__ void __launch_bounds__(256) k_recur_fwd(const Args p) {
   __shared__ float4 map[kWarps][32];   // (a, b) of two channels
-  __shared__ float2 state[32];
+  __shared__ Joint joint;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int groups = p.HD / kGroup, bb = blockIdx.x / groups, cg = blockIdx.x % groups;
-  const int ch = cg * kGroup + 2 * lane;
+  const Place at = take_tile(p);
+  const int groups = p.HD / kGroup, bb = at.chain / groups, cg = at.chain % groups;
+  const int ch = cg * kGroup + 2 * lane, t0 = at.k * kTile + warp * kRows;
   const size_t row0 = (size_t)bb * p.T;
-  if (warp == 0)
-    state[lane] = p.h0 ? *reinterpret_cast<const float2*>(p.h0 + (size_t)bb * p.HD + ch)
-                       : make_float2(0.f, 0.f);
-  for (int tile = 0; tile < p.tiles; ++tile) {
-    const int t0 = tile * kTile + warp * kRows;
-    float2 a[kRows], x[kRows];
-    float4 m = make_float4(1.f, 0.f, 1.f, 0.f);
+  float2 a[kRows], x[kRows];
+  float4 m = make_float4(1.f, 0.f, 1.f, 0.f);
 #pragma unroll
-    for (int r = 0; r < kRows; ++r) {
-      a[r] = make_float2(1.f, 1.f);
-      x[r] = make_float2(0.f, 0.f);
-      if (t0 + r < p.T) {
-        const size_t at = (row0 + t0 + r) * p.HD + ch;
-        const float2 v = ld2(static_cast<const T*>(p.v) + at);
-        const float2 w = ld2(static_cast<const T*>(p.w) + at);
-        a[r] = decay2(ld2(static_cast<const T*>(p.g) + at), p.raw);
-        if constexpr (SAVE8) {
-          put_int8(v, p.v8 + at, p.vs + at / kGroup, lane);
-          put_int8(w, p.w8 + at, p.ws + at / kGroup, lane);
-        }
-        const float2 y = gate2(w, p.raw);
-        x[r] = make_float2(y.x * v.x, y.y * v.y);
+  for (int r = 0; r < kRows; ++r) {
+    a[r] = make_float2(1.f, 1.f);
+    x[r] = make_float2(0.f, 0.f);
+    if (t0 + r < p.T) {
+      const size_t i = (row0 + t0 + r) * p.HD + ch;
+      const float2 v = ld2(static_cast<const T*>(p.v) + i);
+      const float2 w = ld2(static_cast<const T*>(p.w) + i);
+      a[r] = decay2(ld2(static_cast<const T*>(p.g) + i), p.raw);
+      if constexpr (SAVE8) {
+        put_int8(v, p.v8 + i, p.vs + i / kGroup, lane);
+        put_int8(w, p.w8 + i, p.ws + i / kGroup, lane);
       }
-      m.x *= a[r].x; m.y = fmaf(a[r].x, m.y, x[r].x);
-      m.z *= a[r].y; m.w = fmaf(a[r].y, m.w, x[r].y);
+      const float2 y = gate2(w, p.raw);
+      x[r] = make_float2(y.x * v.x, y.y * v.y);
     }
-    map[warp][lane] = m;
-    __syncthreads();
-    float2 h = state[lane];
-    if (warp == 0 && p.kept)
-      *reinterpret_cast<float2*>(p.kept + ((size_t)bb * p.tiles + tile) * p.HD + ch) = h;
-    for (int j = 0; j < warp; ++j) {
-      const float4 z = map[j][lane];
-      h.x = fmaf(z.x, h.x, z.y);
-      h.y = fmaf(z.z, h.y, z.w);
-    }
+    m = after(make_float4(a[r].x, x[r].x, a[r].y, x[r].y), m);
+  }
+  map[warp][lane] = m;
+  __syncthreads();
+  float2 h = enter_tile(p, at, map, joint, p.h0);
+  if (warp == 0 && p.kept)
+    *reinterpret_cast<float2*>(p.kept + ((size_t)bb * p.tiles + at.k) * p.HD + ch) = h;
+  for (int j = 0; j < warp; ++j) h = apply(map[j][lane], h);
 #pragma unroll
-    for (int r = 0; r < kRows; ++r) {
-      h.x = fmaf(a[r].x, h.x, x[r].x);
-      h.y = fmaf(a[r].y, h.y, x[r].y);
-      if (t0 + r < p.T) st2(p.o + (row0 + t0 + r) * p.HD + ch, h);
-      if (t0 + r == p.T - 1) *reinterpret_cast<float2*>(p.hf + (size_t)bb * p.HD + ch) = h;
-    }
-    __syncthreads();
-    if (warp == kWarps - 1) state[lane] = h;
+  for (int r = 0; r < kRows; ++r) {
+    h = apply(make_float4(a[r].x, x[r].x, a[r].y, x[r].y), h);
+    if (t0 + r < p.T) st2(p.o + (row0 + t0 + r) * p.HD + ch, h);
+    if (t0 + r == p.T - 1) *reinterpret_cast<float2*>(p.hf + (size_t)bb * p.HD + ch) = h;
   }
 }
 
+// Tiles in the order of the reverse scan: k = 0 is the last one in time, and the
+// maps of its warps are kept from the last warp to the first.
 template <typename T, bool FROM8>
 __global__ void __launch_bounds__(256) k_recur_bwd(const Args p) {
   __shared__ float4 fmap[kWarps][32], rmap[kWarps][32];
-  __shared__ float2 carry[32];
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int groups = p.HD / kGroup, bb = blockIdx.x / groups, cg = blockIdx.x % groups;
-  const int ch = cg * kGroup + 2 * lane;
+  __shared__ Joint joint;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, back = kWarps - 1 - warp;
+  const Place at = take_tile(p);
+  const int groups = p.HD / kGroup, bb = at.chain / groups, cg = at.chain % groups;
+  const int tile = p.tiles - 1 - at.k;
+  const int ch = cg * kGroup + 2 * lane, t0 = tile * kTile + warp * kRows;
   const size_t row0 = (size_t)bb * p.T;
-  if (warp == 0)
-    carry[lane] = p.dhf ? *reinterpret_cast<const float2*>(p.dhf + (size_t)bb * p.HD + ch)
-                        : make_float2(0.f, 0.f);
-  for (int tile = p.tiles - 1; tile >= 0; --tile) {
-    const int t0 = tile * kTile + warp * kRows;
-    float2 a[kRows], v[kRows], w[kRows], d[kRows], sg[kRows];
+  float2 h = *reinterpret_cast<const float2*>(p.kept + ((size_t)bb * p.tiles + tile) * p.HD + ch);
+  float2 a[kRows], v[kRows], w[kRows], d[kRows], sg[kRows];
 #pragma unroll
-    for (int r = 0; r < kRows; ++r) {
-      a[r] = make_float2(1.f, 1.f);
-      v[r] = w[r] = d[r] = sg[r] = make_float2(0.f, 0.f);
-      if (t0 + r < p.T) {
-        const size_t at = (row0 + t0 + r) * p.HD + ch;
-        if constexpr (FROM8) {
-          const float vs = p.vs[at / kGroup], ws = p.ws[at / kGroup];
-          v[r] = ld2(p.v8 + at);
-          w[r] = ld2(p.w8 + at);
-          v[r].x *= vs; v[r].y *= vs;
-          w[r].x *= ws; w[r].y *= ws;
-        } else {
-          v[r] = ld2(static_cast<const T*>(p.v) + at);
-          w[r] = ld2(static_cast<const T*>(p.w) + at);
-        }
-        sg[r] = ld2(static_cast<const T*>(p.g) + at);
-        a[r] = decay2(sg[r], p.raw);
-        w[r] = gate2(w[r], p.raw);
-        d[r] = ld2(p.dout + at);
+  for (int r = 0; r < kRows; ++r) {
+    a[r] = make_float2(1.f, 1.f);
+    v[r] = w[r] = d[r] = sg[r] = make_float2(0.f, 0.f);
+    if (t0 + r < p.T) {
+      const size_t i = (row0 + t0 + r) * p.HD + ch;
+      if constexpr (FROM8) {
+        const float vs = p.vs[i / kGroup], ws = p.ws[i / kGroup];
+        v[r] = ld2(p.v8 + i);
+        w[r] = ld2(p.w8 + i);
+        v[r].x *= vs; v[r].y *= vs;
+        w[r].x *= ws; w[r].y *= ws;
+      } else {
+        v[r] = ld2(static_cast<const T*>(p.v) + i);
+        w[r] = ld2(static_cast<const T*>(p.w) + i);
       }
+      sg[r] = ld2(static_cast<const T*>(p.g) + i);
+      a[r] = decay2(sg[r], p.raw);
+      w[r] = gate2(w[r], p.raw);
+      d[r] = ld2(p.dout + i);
     }
-    float4 m = make_float4(1.f, 0.f, 1.f, 0.f), n = m;
-#pragma unroll
-    for (int r = 0; r < kRows; ++r) {
-      m.x *= a[r].x; m.y = fmaf(a[r].x, m.y, w[r].x * v[r].x);
-      m.z *= a[r].y; m.w = fmaf(a[r].y, m.w, w[r].y * v[r].y);
-    }
-#pragma unroll
-    for (int r = kRows - 1; r >= 0; --r) {
-      n.y = a[r].x * (d[r].x + n.y);
-      n.w = a[r].y * (d[r].y + n.w);
-    }
-    n.x = m.x;
-    n.z = m.z;
-    fmap[warp][lane] = m;
-    rmap[warp][lane] = n;
-    __syncthreads();
-    float2 h = *reinterpret_cast<const float2*>(p.kept + ((size_t)bb * p.tiles + tile) * p.HD + ch);
-    for (int j = 0; j < warp; ++j) {
-      const float4 z = fmap[j][lane];
-      h.x = fmaf(z.x, h.x, z.y);
-      h.y = fmaf(z.z, h.y, z.w);
-    }
-    float2 c = carry[lane];
-    for (int j = kWarps - 1; j > warp; --j) {
-      const float4 z = rmap[j][lane];
-      c.x = fmaf(z.x, c.x, z.y);
-      c.y = fmaf(z.z, c.y, z.w);
-    }
-    float2 before[kRows];
-#pragma unroll
-    for (int r = 0; r < kRows; ++r) {
-      before[r] = h;
-      h.x = fmaf(a[r].x, h.x, w[r].x * v[r].x);
-      h.y = fmaf(a[r].y, h.y, w[r].y * v[r].y);
-    }
-#pragma unroll
-    for (int r = kRows - 1; r >= 0; --r) {
-      const float2 dh = make_float2(d[r].x + c.x, d[r].y + c.y);
-      c = make_float2(a[r].x * dh.x, a[r].y * dh.y);
-      if (t0 + r < p.T) {
-        const size_t at = (row0 + t0 + r) * p.HD + ch;
-        float2 dw = make_float2(v[r].x * dh.x, v[r].y * dh.y);
-        float2 dg = make_float2(before[r].x * c.x, before[r].y * c.y);
-        if (p.raw) {
-          // d sigmoid(x) = w (1 - w); dg/dx = -sigmoid(x)
-          dw.x *= w[r].x * (1.f - w[r].x);
-          dw.y *= w[r].y * (1.f - w[r].y);
-          dg.x *= -sig_from(expf(-fabsf(sg[r].x)), sg[r].x > 0.f);
-          dg.y *= -sig_from(expf(-fabsf(sg[r].y)), sg[r].y > 0.f);
-        }
-        st2(static_cast<T*>(p.dv) + at, make_float2(w[r].x * dh.x, w[r].y * dh.y));
-        st2(static_cast<T*>(p.dw) + at, dw);
-        st2(static_cast<T*>(p.dg) + at, dg);
-      }
-    }
-    __syncthreads();
-    if (warp == 0) carry[lane] = c;
-    __syncthreads();
   }
-  if (warp == 0)
-    *reinterpret_cast<float2*>(p.dh0 + (size_t)bb * p.HD + ch) = carry[lane];
+  float4 m = make_float4(1.f, 0.f, 1.f, 0.f), n = m;
+#pragma unroll
+  for (int r = 0; r < kRows; ++r)
+    m = after(make_float4(a[r].x, w[r].x * v[r].x, a[r].y, w[r].y * v[r].y), m);
+#pragma unroll
+  for (int r = kRows - 1; r >= 0; --r) {
+    n.y = a[r].x * (d[r].x + n.y);
+    n.w = a[r].y * (d[r].y + n.w);
+  }
+  n.x = m.x;
+  n.z = m.z;
+  fmap[warp][lane] = m;
+  rmap[back][lane] = n;
+  __syncthreads();
+  float2 c = enter_tile(p, at, rmap, joint, p.dhf);
+  for (int j = 0; j < warp; ++j) h = apply(fmap[j][lane], h);
+  for (int j = 0; j < back; ++j) c = apply(rmap[j][lane], c);
+  float2 before[kRows];
+#pragma unroll
+  for (int r = 0; r < kRows; ++r) {
+    before[r] = h;
+    h = apply(make_float4(a[r].x, w[r].x * v[r].x, a[r].y, w[r].y * v[r].y), h);
+  }
+#pragma unroll
+  for (int r = kRows - 1; r >= 0; --r) {
+    const float2 dh = make_float2(d[r].x + c.x, d[r].y + c.y);
+    c = make_float2(a[r].x * dh.x, a[r].y * dh.y);
+    if (t0 + r < p.T) {
+      const size_t i = (row0 + t0 + r) * p.HD + ch;
+      float2 dw = make_float2(v[r].x * dh.x, v[r].y * dh.y);
+      float2 dg = make_float2(before[r].x * c.x, before[r].y * c.y);
+      if (p.raw) {
+        // d sigmoid(x) = w (1 - w); dg/dx = -sigmoid(x)
+        dw.x *= w[r].x * (1.f - w[r].x);
+        dw.y *= w[r].y * (1.f - w[r].y);
+        dg.x *= -sig_from(expf(-fabsf(sg[r].x)), sg[r].x > 0.f);
+        dg.y *= -sig_from(expf(-fabsf(sg[r].y)), sg[r].y > 0.f);
+      }
+      st2(static_cast<T*>(p.dv) + i, make_float2(w[r].x * dh.x, w[r].y * dh.y));
+      st2(static_cast<T*>(p.dw) + i, dw);
+      st2(static_cast<T*>(p.dg) + i, dg);
+    }
+  }
+  if (tile == 0 && warp == 0) *reinterpret_cast<float2*>(p.dh0 + (size_t)bb * p.HD + ch) = c;
 }
 
 int check(int dtype, int B, int T, int H, int D) {
@@ -249,18 +342,25 @@ int check(int dtype, int B, int T, int H, int D) {
     return report_error(GDN2_ERR_INVALID, "gdn2_recur: empty problem B*T*H");
   if (D != 64 && D != 128 && D != 256)
     return report_error(GDN2_ERR_INVALID, "gdn2_recur: head dim D unsupported (64, 128 or 256)");
-  if (T > (1 << 30) || (long)H * D > (1 << 24) || (long)B * H * D / kGroup > 0x7fffffffL)
+  const long chains = (long)B * ((long)H * (D / kGroup));
+  if (T > (1 << 30) || (long)H * D > (1 << 24) || chains > (1 << 26) ||
+      chains * ((T + kTile - 1) / kTile) > 0x7fffffffL)
     return report_error(GDN2_ERR_INVALID, "gdn2_recur: too many tokens or channels");
   return GDN2_OK;
 }
 
 bool misaligned(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) != 0; }
 
-// The status header that gdn2_workspace_status() reads, cleared as by every
-// entry point that takes a workspace.
-int clear_status(void* workspace, cudaStream_t s) {
-  char* hdr = reinterpret_cast<char*>((reinterpret_cast<uintptr_t>(workspace) + 255) & ~(uintptr_t)255);
-  const cudaError_t e = cudaMemsetAsync(hdr, 0, 256, s);
+// Zeroes the scratch: the status header that gdn2_workspace_status() reads, the
+// tile counter and every published word.
+int prepare(Args& p, int B, void* workspace, cudaStream_t s) {
+  p.chains = B * (p.HD / kGroup);
+  if (p.tiles == 1) return GDN2_OK;
+  char* base = reinterpret_cast<char*>((reinterpret_cast<uintptr_t>(workspace) + 255) & ~(uintptr_t)255);
+  p.s.status = reinterpret_cast<int*>(base);
+  p.s.maps = reinterpret_cast<ulonglong2*>(base + 256);
+  p.s.enter = p.s.maps + (size_t)p.tiles * p.chains * 32;
+  const cudaError_t e = cudaMemsetAsync(base, 0, scratch_bytes(p.tiles, p.chains) - 256, s);
   return e == cudaSuccess ? GDN2_OK : report_error(GDN2_ERR_CUDA, cudaGetErrorString(e));
 }
 
@@ -278,7 +378,7 @@ extern "C" size_t gdn2_recur_kept_floats(int B, int T, int H, int D) {
 
 extern "C" size_t gdn2_recur_workspace_bytes(int B, int T, int H, int D) {
   if (check(GDN2_F32, B, T, H, D)) return 0;
-  return 512;
+  return scratch_bytes((T + kTile - 1) / kTile, (size_t)B * H * D / kGroup);
 }
 
 extern "C" int gdn2_recur_fwd(int dtype, const void* v, const void* w, const void* g,
@@ -303,11 +403,9 @@ extern "C" int gdn2_recur_fwd(int dtype, const void* v, const void* w, const voi
   p.vs = v_scales; p.ws = w_scales;
   p.T = T; p.HD = H * D; p.tiles = (T + kTile - 1) / kTile; p.raw = raw;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  if (T > kTile) {
-    const int e = clear_status(workspace, s);
-    if (e) return e;
-  }
-  const unsigned grid = (unsigned)((size_t)B * H * D / kGroup);
+  const int e = prepare(p, B, workspace, s);
+  if (e) return e;
+  const unsigned grid = (unsigned)((size_t)p.chains * p.tiles);
   if (dtype == GDN2_F32) {
     if (save8) k_recur_fwd<float, true><<<grid, 256, 0, s>>>(p);
     else k_recur_fwd<float, false><<<grid, 256, 0, s>>>(p);
@@ -348,11 +446,9 @@ extern "C" int gdn2_recur_bwd(int dtype, const void* v, const void* w, const voi
   p.dv = dv; p.dw = dw; p.dg = dg; p.dh0 = dh0;
   p.T = T; p.HD = H * D; p.tiles = (T + kTile - 1) / kTile; p.raw = raw;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  if (T > kTile) {
-    const int e = clear_status(workspace, s);
-    if (e) return e;
-  }
-  const unsigned grid = (unsigned)((size_t)B * H * D / kGroup);
+  const int e = prepare(p, B, workspace, s);
+  if (e) return e;
+  const unsigned grid = (unsigned)((size_t)p.chains * p.tiles);
   if (dtype == GDN2_F32) {
     if (from8) k_recur_bwd<float, true><<<grid, 256, 0, s>>>(p);
     else k_recur_bwd<float, false><<<grid, 256, 0, s>>>(p);
