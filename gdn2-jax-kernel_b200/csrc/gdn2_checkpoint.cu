@@ -55,20 +55,30 @@ template <> struct Vec<__nv_bfloat16> {
   }
 };
 
-// Codes of E values, one word per 4.  Every lane of the group's 64 / E calls.
+constexpr int kUnroll = 4;   // 16-byte pieces a thread holds at once
+
+// Codes of the kUnroll pieces of a thread, one word per 4 values, and in `scale`
+// the scale of piece (lane & 3): a group's lanes share its division (every lane
+// dividing for every piece cost a third of the instructions).  Whole warps call.
 template <int E>
-__device__ __forceinline__ float encode(const float (&x)[E], unsigned (&word)[E / 4]) {
-  unsigned top = 0;
+__device__ __forceinline__ float encode(const float (&x)[kUnroll][E], unsigned (&word)[kUnroll][E / 4]) {
+  float mine = 0.f;
 #pragma unroll
-  for (int i = 0; i < E; ++i) top = max(top, abs_bits(x[i]));
+  for (int u = 0; u < kUnroll; ++u) {
+    float top = fabsf(x[u][0]);
 #pragma unroll
-  for (int o = 1; o < kGroup / E; o <<= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
-  const GroupScale s = group_scale(top);
+    for (int i = 1; i < E; ++i) top = max_abs(top, x[u][i]);
 #pragma unroll
-  for (int i = 0; i < E; i += 4)
-    word[i / 4] = pack4(int8_code(x[i], s), int8_code(x[i + 1], s), int8_code(x[i + 2], s),
-                        int8_code(x[i + 3], s));
-  return s.scale;
+    for (int o = 1; o < kGroup / E; o <<= 1)
+      top = max_abs(top, __shfl_xor_sync(0xffffffffu, top, o));
+    const float inv = group_inv(top);
+    unsigned c[E];
+    int8_codes<E>(x[u], inv, top, c);
+#pragma unroll
+    for (int i = 0; i < E; i += 4) word[u][i / 4] = pack4(c[i], c[i + 1], c[i + 2], c[i + 3]);
+    if ((threadIdx.x & 3) == u) mine = top;
+  }
+  return group_scale(mine);
 }
 template <int E>
 __device__ __forceinline__ void decode(float (&x)[E], const unsigned (&word)[E / 4], float scale) {
@@ -92,7 +102,15 @@ __device__ __forceinline__ void st_words(int8_t* p, const unsigned (&w)[E / 4]) 
   else *reinterpret_cast<uint2*>(p) = make_uint2(w[0], w[1]);
 }
 
-constexpr int kUnroll = 4;   // 16-byte pieces a thread holds at once
+// Lane u of a group (u < kUnroll) stores the scale of the group's piece u: value
+// index of that piece for this lane, or no index.
+template <int E>
+__device__ __forceinline__ bool scale_place(size_t base, size_t n, size_t& group) {
+  const int lane = threadIdx.x % (kGroup / E);
+  const size_t i = base + (size_t)lane * 256 * E;
+  group = i / kGroup;
+  return lane < kUnroll && i < n;
+}
 
 // blockIdx.y: tensor; n: values of each (a multiple of 64).  The bounds are
 // per thread, but a group's lanes are in or out of them together.
@@ -109,16 +127,15 @@ __global__ void __launch_bounds__(256) k_pack(Tensors a, size_t n) {
     const size_t i = base + (size_t)u * 256 * E;
     if (i < n) Vec<T>::load(v[u], x + i);
   }
+  unsigned w[kUnroll][E / 4];
+  const float scale = encode<E>(v, w);
 #pragma unroll
   for (int u = 0; u < kUnroll; ++u) {
     const size_t i = base + (size_t)u * 256 * E;
-    unsigned w[E / 4];
-    const float scale = encode<E>(v[u], w);
-    if (i < n) {
-      st_words<E>(c + i, w);
-      if (i % kGroup == 0) s[i / kGroup] = scale;
-    }
+    if (i < n) st_words<E>(c + i, w[u]);
   }
+  size_t group;
+  if (scale_place<E>(base, n, group)) s[group] = scale;
 }
 
 template <typename T>
@@ -171,17 +188,18 @@ k_state_write(const float* __restrict__ h, int8_t* __restrict__ codes, float* __
   int8_t* c = codes + (size_t)slot * n;
   float* s = scales + (size_t)slot * (n / kGroup);
 #pragma unroll
-  for (int u = 0; u < kUnroll; ++u) {
-    const size_t i = base + (size_t)u * 256 * E;
+  for (int u = 0; u < kUnroll; ++u)
 #pragma unroll
     for (int k = 0; k < E; ++k) v[u][k] = san(v[u][k], clip);
-    unsigned w[1];
-    const float scale = encode<E>(v[u], w);
-    if (i < n) {
-      st_words<E>(c + i, w);
-      if (i % kGroup == 0) s[i / kGroup] = scale;
-    }
+  unsigned w[kUnroll][1];
+  const float scale = encode<E>(v, w);
+#pragma unroll
+  for (int u = 0; u < kUnroll; ++u) {
+    const size_t i = base + (size_t)u * 256 * E;
+    if (i < n) st_words<E>(c + i, w[u]);
   }
+  size_t group;
+  if (scale_place<E>(base, n, group)) s[group] = scale;
 }
 
 // A slot of -1 reads as the zero state; one outside the cache as NaN.

@@ -139,19 +139,19 @@ k_decode_cached(const T* __restrict__ q, const T* __restrict__ k, const T* __res
   if (to < 0) return;
 #pragma unroll
   for (int r = 0; r < R; ++r) {
-    unsigned top = 0;
+    float top = fabsf(s[r][0]);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) top = max(top, abs_bits(s[r][i]));
+    for (int i = 1; i < 8; ++i) top = max_abs(top, s[r][i]);
 #pragma unroll
-    for (int x = 1; x < 8; x <<= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, x));
-    const GroupScale gs = group_scale(top);
+    for (int x = 1; x < 8; x <<= 1) top = max_abs(top, __shfl_xor_sync(0xffffffffu, top, x));
+    const float inv = group_inv(top);
     uint2 c;
-    auto code = [&](int i) { return int8_code_near(s[r][i], gs.inv); };
+    auto code = [&](int i) { return int8_code_near(s[r][i], inv); };
     c.x = pack4(code(0), code(1), code(2), code(3));
     c.y = pack4(code(4), code(5), code(6), code(7));
     const size_t at = (((size_t)to * H + h) * D + (r * NW + warp) * RW + rl);
     *reinterpret_cast<uint2*>(codes + at * D + cl * 8) = c;
-    if (cl % 8 == 0) scales[at * G + cl * 8 / kGroup] = gs.scale;
+    if (cl % 8 == 0) scales[at * G + cl * 8 / kGroup] = group_scale(top);
   }
 }
 

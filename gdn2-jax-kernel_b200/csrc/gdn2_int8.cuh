@@ -25,41 +25,63 @@ constexpr float kInt8Tiny = 0x1p-100f;
 // an integer maximum keeps NaN (a float maximum would drop it).
 __device__ __forceinline__ unsigned abs_bits(float x) { return __float_as_uint(x) & 0x7fffffffu; }
 
-struct GroupScale {
-  float top, inv, scale;   // max|x|, 127 / max|x| (0: every code is 0), max|x| / 127
-};
-__device__ __forceinline__ GroupScale group_scale(unsigned top_bits) {
-  GroupScale s;
-  s.top = __uint_as_float(top_bits);
-  const bool fits = top_bits < 0x7f800000u, some = s.top >= kInt8Tiny;
-  s.inv = fits && some ? __fdiv_rn(127.f, s.top) : 0.f;
-  s.scale = !fits ? __uint_as_float(0x7fc00000u) : some ? __fdiv_rn(s.top, 127.f) : 0.f;
-  return s;
+// max|x|, |y| that keeps a NaN.
+__device__ __forceinline__ float max_abs(float x, float y) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(fabsf(x)), "f"(fabsf(y)));
+  return r;
 }
 
-// y = x * inv is off by at most 127 * 2^-23 = 1.5e-5, so only a y within 1e-4
-// of a half can round the wrong way; there 254 |x| is compared with
-// (2 floor + 1) * top, both exact in float64 (24 + 8 bits).  One value in 5000
-// takes this path.
+// 127 / top for the codes, to 2^-22.5 of itself (what that leaves open,
+// int8_code4 decides); 0, so that every code is 0, for a group without a scale.
+__device__ __forceinline__ float group_inv(float top) {
+  float r;
+  asm("rcp.approx.f32 %0, %1;" : "=f"(r) : "f"(top));
+  return top >= kInt8Tiny && top <= 3.402823466e38f ? 127.f * r : 0.f;
+}
+// The stored scale, rounded once.
+__device__ __forceinline__ float group_scale(float top) {
+  return !(top <= 3.402823466e38f) ? __uint_as_float(0x7fc00000u)
+         : top >= kInt8Tiny ? __fdiv_rn(top, 127.f) : 0.f;
+}
+
+// 254 |x| against (2 floor + 1) * top, both exact in float64 (24 + 8 bits).
 static __device__ __noinline__ float int8_border(float x, float y, float top) {
   const float lo = floorf(fabsf(y));
   const double l = 254.0 * (double)fabsf(x), r = (2.0 * (double)lo + 1.0) * (double)top;
   const bool up = l > r || (l == r && ((int)lo & 1));
   return copysignf(lo + (up ? 1.f : 0.f), x);
 }
-__device__ __forceinline__ int int8_code(float x, const GroupScale& s) {
-  const float y = x * s.inv;
-  float r = rintf(y);
-  if (fabsf(y - r) > 0.4999f) r = int8_border(x, y, s.top);
-  return __float2int_rn(r);   // NaN (inv = 0 times an infinity) gives 0
+// The codes of N values of one group, each in the low byte of a word.
+// 1.5 * 2^23 added to |y| <= 127.01 rounds y = x * inv to a whole number, in the
+// low bits (the conversion and rounding instructions run at an eighth of the
+// rate).  y is off by at most 127 * 2^-22.5 = 2.2e-5, so only a y within 1e-4 of
+// a half can round the wrong way: one value in 5000 is decided in float64.
+template <int N>
+__device__ __forceinline__ void int8_codes(const float (&x)[N], float inv, float top,
+                                           unsigned (&code)[N]) {
+  float far = 0.f;
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    const float t = fmaf(x[i], inv, 12582912.f);
+    far = fmaxf(far, fabsf(fmaf(x[i], inv, 12582912.f - t)));
+    code[i] = __float_as_uint(t);
+  }
+  if (far > 0.4999f) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const float y = x[i] * inv, r = __uint_as_float(code[i]) - 12582912.f;
+      if (fabsf(y - r) > 0.4998f)
+        code[i] = __float_as_uint(int8_border(x[i], y, top) + 12582912.f);
+    }
+  }
 }
 // The nearest code by float32 arithmetic alone, for values that carry rounding
-// errors of their own: off from a half step by at most 1.5e-5 of a step.
-// 1.5 * 2^23 added to |y| <= 127.01 leaves rint(y) in the low byte.
+// errors of their own: off from a half step by at most 2.2e-5 of a step.
 __device__ __forceinline__ unsigned int8_code_near(float x, float inv) {
   return __float_as_uint(fmaf(x, inv, 12582912.f));
 }
-__device__ __forceinline__ unsigned pack4(int a, int b, int c, int d) {
+__device__ __forceinline__ unsigned pack4(unsigned a, unsigned b, unsigned c, unsigned d) {
   return __byte_perm(__byte_perm(a, b, 0x0040), __byte_perm(c, d, 0x0040), 0x5410);
 }
 // Byte I of four codes as a float: the code moved to 0..255 becomes the low

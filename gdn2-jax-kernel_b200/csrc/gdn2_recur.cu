@@ -33,6 +33,8 @@
 // those of the restored values, restarted from the true state every 64 tokens.
 // Decays stay in their own type: a rounding of a log decay compounds over the
 // sequence, one of v or w does not.
+#include <type_traits>
+
 #include "../../include/gdn2.h"
 #include "gdn2_int8.cuh"
 
@@ -49,15 +51,49 @@ constexpr int kWarps = 8;
 constexpr int kTile = kRows * kWarps;    // tokens of a tile: the interval of the kept states
 static_assert(kTile == GDN2_RECUR_INTERVAL, "interval of the kept states");
 
-// Two neighbouring channels.
-__device__ __forceinline__ float2 ld2(const float* p) { return __ldcs(reinterpret_cast<const float2*>(p)); }
-__device__ __forceinline__ float2 ld2(const __nv_bfloat16* p) {
-  const unsigned u = __ldcs(reinterpret_cast<const unsigned*>(p));
+// Two neighbouring channels, as one operand of the packed float32 instructions.
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+  float2 d;
+  asm("{.reg .b64 x, y, z;\n\t"
+      "mov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\tmov.b64 z, {%6, %7};\n\t"
+      "fma.rn.f32x2 x, x, y, z;\n\tmov.b64 {%0, %1}, x;}"
+      : "=f"(d.x), "=f"(d.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+  return d;
+}
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+  float2 d;
+  asm("{.reg .b64 x, y;\n\t"
+      "mov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\t"
+      "mul.rn.f32x2 x, x, y;\n\tmov.b64 {%0, %1}, x;}"
+      : "=f"(d.x), "=f"(d.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return d;
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+  float2 d;
+  asm("{.reg .b64 x, y;\n\t"
+      "mov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\t"
+      "add.rn.f32x2 x, x, y;\n\tmov.b64 {%0, %1}, x;}"
+      : "=f"(d.x), "=f"(d.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return d;
+}
+__device__ __forceinline__ float2 both(float x) { return make_float2(x, x); }
+
+// As loaded: what a row of two channels is before it is converted.
+template <typename T> struct Raw;
+template <> struct Raw<float> { using type = float2; };
+template <> struct Raw<__nv_bfloat16> { using type = unsigned; };
+template <> struct Raw<int8_t> { using type = unsigned short; };
+template <typename T>
+__device__ __forceinline__ typename Raw<T>::type ldraw(const T* p) {
+  return __ldcs(reinterpret_cast<const typename Raw<T>::type*>(p));
+}
+__device__ __forceinline__ float2 value2(float2 v) { return v; }
+__device__ __forceinline__ float2 value2(unsigned u) {
   return make_float2(__uint_as_float(u << 16), __uint_as_float(u & 0xffff0000u));
 }
-__device__ __forceinline__ float2 ld2(const int8_t* p) {
-  const short u = __ldcs(reinterpret_cast<const short*>(p));
-  return make_float2((float)(int8_t)(u & 0xff), (float)(int8_t)(u >> 8));
+__device__ __forceinline__ float2 value2(unsigned short u) {
+  const unsigned b = u ^ 0x8080u;
+  return make_float2(code_f<0>(b), code_f<1>(b));
 }
 __device__ __forceinline__ void st2(float* p, float2 v) { __stcs(reinterpret_cast<float2*>(p), v); }
 __device__ __forceinline__ void st2(__nv_bfloat16* p, float2 v) {
@@ -68,26 +104,25 @@ __device__ __forceinline__ void st2(__nv_bfloat16* p, float2 v) {
 // e^g, or from the pre-activation x of g = -softplus(x): sigmoid(-x), from
 // e^{-|x|} so that neither end overflows or cancels.
 __device__ __forceinline__ float sig_from(float e, bool high) { return (high ? 1.f : e) / (1.f + e); }
-__device__ __forceinline__ float decay(float g, int raw) {
-  return raw ? sig_from(expf(-fabsf(g)), g < 0.f) : expf(g);
+__device__ __forceinline__ float sig(float x) { return sig_from(expf(-fabsf(x)), x > 0.f); }
+template <bool RAW>
+__device__ __forceinline__ float2 decay2(float2 g) {
+  return RAW ? make_float2(sig(-g.x), sig(-g.y)) : make_float2(expf(g.x), expf(g.y));
 }
-__device__ __forceinline__ float2 decay2(float2 g, int raw) {
-  return make_float2(decay(g.x, raw), decay(g.y, raw));
-}
-__device__ __forceinline__ float2 gate2(float2 w, int raw) {
-  return raw ? make_float2(gate_sig(w.x), gate_sig(w.y)) : w;
-}
-
-// The int8 form of one group (a warp's 64 channels) of a row.
-__device__ __forceinline__ void put_int8(float2 x, int8_t* codes, float* scale, int lane) {
-  const unsigned top = __reduce_max_sync(0xffffffffu, max(abs_bits(x.x), abs_bits(x.y)));
-  const GroupScale s = group_scale(top);
-  const int a = int8_code(x.x, s), b = int8_code(x.y, s);
-  *reinterpret_cast<short*>(codes) = (short)((a & 0xff) | (b << 8));
-  if (lane == 0) *scale = s.scale;
+template <bool RAW>
+__device__ __forceinline__ float2 gate2(float2 w) {
+  return RAW ? make_float2(sig(w.x), sig(w.y)) : w;
 }
 
-constexpr int kGroupTiles = 16;
+// A map h -> a h + b of two channels.
+struct Map { float2 a, b; };
+__device__ __forceinline__ Map identity() { return {both(1.f), both(0.f)}; }
+__device__ __forceinline__ Map after(Map m2, Map m1) { return {mul2(m2.a, m1.a), fma2(m2.a, m1.b, m2.b)}; }
+__device__ __forceinline__ float2 apply(Map m, float2 h) { return fma2(m.a, h, m.b); }
+__device__ __forceinline__ float4 flat(Map m) { return make_float4(m.a.x, m.a.y, m.b.x, m.b.y); }
+__device__ __forceinline__ Map unflat(float4 f) { return {make_float2(f.x, f.y), make_float2(f.z, f.w)}; }
+
+constexpr int kGroupTiles = 2 * kWarps;
 constexpr int kPolls = 1 << 22;   // about two seconds, then the status word is set
 
 // Scratch of one call with more than one tile, zeroed before the kernel.
@@ -103,9 +138,9 @@ size_t scratch_bytes(size_t tiles, size_t chains) {
 __device__ __forceinline__ unsigned long long word(float a, float b) {
   return ((unsigned long long)__float_as_uint(b) << 32) | (__float_as_uint(a) | 0x80000000u);
 }
-__device__ __forceinline__ void publish(ulonglong2* p, float4 m) {
+__device__ __forceinline__ void publish(ulonglong2* p, Map m) {
   asm volatile("st.relaxed.gpu.global.v2.u64 [%0], {%1, %2};"
-               ::"l"(p), "l"(word(m.x, m.y)), "l"(word(m.z, m.w)) : "memory");
+               ::"l"(p), "l"(word(m.a.x, m.b.x)), "l"(word(m.a.y, m.b.y)) : "memory");
 }
 __device__ __forceinline__ ulonglong2 peek(const ulonglong2* p) {
   ulonglong2 v;
@@ -113,14 +148,14 @@ __device__ __forceinline__ ulonglong2 peek(const ulonglong2* p) {
   return v;
 }
 __device__ __forceinline__ bool there(ulonglong2 v) { return ((unsigned)v.x & (unsigned)v.y) >> 31; }
-__device__ __forceinline__ float4 unword(ulonglong2 v) {
-  return make_float4(__uint_as_float((unsigned)v.x & 0x7fffffffu), __uint_as_float((unsigned)(v.x >> 32)),
-                     __uint_as_float((unsigned)v.y & 0x7fffffffu), __uint_as_float((unsigned)(v.y >> 32)));
+__device__ __forceinline__ Map unword(ulonglong2 v) {
+  return {make_float2(__uint_as_float((unsigned)v.x & 0x7fffffffu), __uint_as_float((unsigned)v.y & 0x7fffffffu)),
+          make_float2(__uint_as_float((unsigned)(v.x >> 32)), __uint_as_float((unsigned)(v.y >> 32)))};
 }
 // Waits until the words at p are there in every lane, kPolls times at most; a
 // wait that runs out, here or elsewhere in the call, is in the status word and
 // ends this one too.
-__device__ float4 await(const ulonglong2* p, int* status) {
+__device__ Map await(const ulonglong2* p, int* status) {
   ulonglong2 v = peek(p);
   for (int i = 1; !__all_sync(0xffffffffu, there(v)); ++i) {
     if (i >= kPolls || (i % 4096 == 0 && *(volatile int*)status)) {
@@ -132,14 +167,6 @@ __device__ float4 await(const ulonglong2* p, int* status) {
   return unword(v);
 }
 
-// m2 after m1, on two channels.
-__device__ __forceinline__ float4 after(float4 m2, float4 m1) {
-  return make_float4(m2.x * m1.x, fmaf(m2.x, m1.y, m2.y), m2.z * m1.z, fmaf(m2.z, m1.w, m2.w));
-}
-__device__ __forceinline__ float2 apply(float4 m, float2 h) {
-  return make_float2(fmaf(m.x, h.x, m.y), fmaf(m.z, h.y, m.w));
-}
-
 struct Args {
   const void *v, *w, *g;
   int8_t *v8, *w8;        // int8 checkpoints, or NULL
@@ -149,7 +176,7 @@ struct Args {
   void *dv, *dw, *dg;
   float* dh0;
   Scratch s;
-  int T, HD, tiles, chains, raw;
+  int T, HD, tiles, chains;
 };
 
 // The tile of this CTA: (chain, index k in the order of the scan).
@@ -177,40 +204,73 @@ __device__ __forceinline__ float2 enter_tile(const Args& p, const Place at,
                                              const float* first) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int mate = at.k % kGroupTiles, group = at.k / kGroupTiles;
-  const bool last = at.k + 1 == p.tiles;
-  if (warp == 0 && !last && mate != kGroupTiles - 1) {
-    float4 m = map[0][lane];
+  const bool last = at.k + 1 == p.tiles, hands_on = mate == kGroupTiles - 1 && !last;
+  if (warp == 0 && !last && !hands_on) {
+    Map m = unflat(map[0][lane]);
 #pragma unroll
-    for (int j = 1; j < kWarps; ++j) m = after(map[j][lane], m);
+    for (int j = 1; j < kWarps; ++j) m = after(unflat(map[j][lane]), m);
     publish(p.s.maps + ((size_t)at.k * p.chains + at.chain) * 32 + lane, m);
   }
-  for (int i = warp; i < mate; i += kWarps)
-    joint.mates[i][lane] =
-        await(p.s.maps + ((size_t)(at.k - mate + i) * p.chains + at.chain) * 32 + lane, p.s.status);
-  if (warp == kWarps - 1) {
-    float2 h = make_float2(0.f, 0.f);
-    if (group) {
-      const float4 m = await(p.s.enter + ((size_t)group * p.chains + at.chain) * 32 + lane, p.s.status);
-      h = make_float2(m.y, m.w);
-    } else if (first) {
-      h = *reinterpret_cast<const float2*>(first + (size_t)at.chain * kGroup + 2 * lane);
+  const ulonglong2* mine = p.s.maps + ((size_t)(at.k - mate) * p.chains + at.chain) * 32 + lane;
+  const size_t next = (size_t)p.chains * 32;
+  if (warp < mate) {   // two waits at once: the second has mostly come when the first has
+    const bool two = warp + kWarps < mate;
+    const ulonglong2 second = two ? peek(mine + (warp + kWarps) * next) : ulonglong2{};
+    joint.mates[warp][lane] = flat(await(mine + warp * next, p.s.status));
+    if (two)
+      joint.mates[warp + kWarps][lane] =
+          flat(__all_sync(0xffffffffu, there(second)) ? unword(second)
+                                                      : await(mine + (warp + kWarps) * next, p.s.status));
+  }
+  if (mate) __syncthreads();
+  if (warp == 0) {
+    // the step from group to group is the dependent one: everything else of it
+    // is joined before the wait
+    Map m = identity();
+    if (hands_on) {
+      for (int i = 0; i < mate; ++i) m = after(unflat(joint.mates[i][lane]), m);
+#pragma unroll
+      for (int j = 0; j < kWarps; ++j) m = after(unflat(map[j][lane]), m);
     }
+    float2 h = both(0.f);
+    if (group)
+      h = await(p.s.enter + ((size_t)group * p.chains + at.chain) * 32 + lane, p.s.status).b;
+    else if (first)
+      h = *reinterpret_cast<const float2*>(first + (size_t)at.chain * kGroup + 2 * lane);
+    if (hands_on)
+      publish(p.s.enter + ((size_t)(group + 1) * p.chains + at.chain) * 32 + lane,
+              {both(0.f), apply(m, h)});
     joint.enter[lane] = h;
   }
   __syncthreads();
   float2 h = joint.enter[lane];
-  for (int i = 0; i < mate; ++i) h = apply(joint.mates[i][lane], h);
-  if (warp == 0 && !last && mate == kGroupTiles - 1) {
-    float2 e = h;
-#pragma unroll
-    for (int j = 0; j < kWarps; ++j) e = apply(map[j][lane], e);
-    publish(p.s.enter + ((size_t)(group + 1) * p.chains + at.chain) * 32 + lane,
-            make_float4(0.f, e.x, 0.f, e.y));
-  }
+  for (int i = 0; i < mate; ++i) h = apply(unflat(joint.mates[i][lane]), h);
   return h;
 }
 
-template <typename T, bool SAVE8>
+// The int8 forms of a warp's 16 groups (8 rows of two tensors): codes are
+// stored here, lane 2 r + j keeps the scale of tensor j's row r (one division a
+// lane instead of one a group).
+__device__ __forceinline__ float put_int8(const float2 (&v)[kRows], const float2 (&w)[kRows],
+                                          int8_t* v8, int8_t* w8, size_t stride, int rows, int lane) {
+  float mine = 0.f;
+#pragma unroll
+  for (int r = 0; r < kRows; ++r) {
+    const float tv = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(max_abs(v[r].x, v[r].y))));
+    const float tw = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(max_abs(w[r].x, w[r].y))));
+    unsigned c[2], d[2];
+    int8_codes<2>({v[r].x, v[r].y}, group_inv(tv), tv, c);
+    int8_codes<2>({w[r].x, w[r].y}, group_inv(tw), tw, d);
+    if (r < rows) {
+      *reinterpret_cast<unsigned short*>(v8 + r * stride) = (unsigned short)__byte_perm(c[0], c[1], 0x0040);
+      *reinterpret_cast<unsigned short*>(w8 + r * stride) = (unsigned short)__byte_perm(d[0], d[1], 0x0040);
+    }
+    mine = lane == 2 * r ? tv : lane == 2 * r + 1 ? tw : mine;
+  }
+  return group_scale(mine);
+}
+
+template <typename T, bool SAVE8, bool RAW>
 __global__ void __launch_bounds__(256) k_recur_fwd(const Args p) {
   __shared__ float4 map[kWarps][32];   // (a, b) of two channels
   __shared__ Joint joint;
@@ -218,45 +278,65 @@ __global__ void __launch_bounds__(256) k_recur_fwd(const Args p) {
   const Place at = take_tile(p);
   const int groups = p.HD / kGroup, bb = at.chain / groups, cg = at.chain % groups;
   const int ch = cg * kGroup + 2 * lane, t0 = at.k * kTile + warp * kRows;
-  const size_t row0 = (size_t)bb * p.T;
+  const int rows = min(kRows, p.T - t0);   // of this warp; below 1: none
+  const size_t i0 = ((size_t)bb * p.T + t0) * p.HD + ch;
   float2 a[kRows], x[kRows];
-  float4 m = make_float4(1.f, 0.f, 1.f, 0.f);
+  if (rows > 0) {
+    // every load before any arithmetic; rows behind the end read the last one
+    typename Raw<T>::type rg[kRows], rv[kRows], rw[kRows];
 #pragma unroll
-  for (int r = 0; r < kRows; ++r) {
-    a[r] = make_float2(1.f, 1.f);
-    x[r] = make_float2(0.f, 0.f);
-    if (t0 + r < p.T) {
-      const size_t i = (row0 + t0 + r) * p.HD + ch;
-      const float2 v = ld2(static_cast<const T*>(p.v) + i);
-      const float2 w = ld2(static_cast<const T*>(p.w) + i);
-      a[r] = decay2(ld2(static_cast<const T*>(p.g) + i), p.raw);
-      if constexpr (SAVE8) {
-        put_int8(v, p.v8 + i, p.vs + i / kGroup, lane);
-        put_int8(w, p.w8 + i, p.ws + i / kGroup, lane);
-      }
-      const float2 y = gate2(w, p.raw);
-      x[r] = make_float2(y.x * v.x, y.y * v.y);
+    for (int r = 0; r < kRows; ++r) {
+      const size_t i = i0 + (size_t)min(r, rows - 1) * p.HD;
+      rg[r] = ldraw(static_cast<const T*>(p.g) + i);
+      rv[r] = ldraw(static_cast<const T*>(p.v) + i);
+      rw[r] = ldraw(static_cast<const T*>(p.w) + i);
     }
-    m = after(make_float4(a[r].x, x[r].x, a[r].y, x[r].y), m);
+    if constexpr (SAVE8) {
+      float2 v[kRows], w[kRows];
+#pragma unroll
+      for (int r = 0; r < kRows; ++r) {
+        v[r] = value2(rv[r]);
+        w[r] = value2(rw[r]);
+      }
+      const float scale = put_int8(v, w, p.v8 + i0, p.w8 + i0, p.HD, rows, lane);
+      if (lane < 2 * rows)
+        (lane & 1 ? p.ws : p.vs)[(i0 - 2 * lane) / kGroup + (size_t)(lane >> 1) * groups] = scale;
+    }
+#pragma unroll
+    for (int r = 0; r < kRows; ++r) {
+      a[r] = decay2<RAW>(value2(rg[r]));
+      x[r] = mul2(gate2<RAW>(value2(rw[r])), value2(rv[r]));
+    }
   }
-  map[warp][lane] = m;
+  if (rows < kRows) {
+#pragma unroll
+    for (int r = 0; r < kRows; ++r)
+      if (r >= rows) a[r] = both(1.f), x[r] = both(0.f);
+  }
+  Map m = {a[0], x[0]};
+#pragma unroll
+  for (int r = 1; r < kRows; ++r) m = after({a[r], x[r]}, m);
+  map[warp][lane] = flat(m);
   __syncthreads();
   float2 h = enter_tile(p, at, map, joint, p.h0);
   if (warp == 0 && p.kept)
     *reinterpret_cast<float2*>(p.kept + ((size_t)bb * p.tiles + at.k) * p.HD + ch) = h;
-  for (int j = 0; j < warp; ++j) h = apply(map[j][lane], h);
+  for (int j = 0; j < warp; ++j) h = apply(unflat(map[j][lane]), h);
+  float* o = p.o + i0;
 #pragma unroll
   for (int r = 0; r < kRows; ++r) {
-    h = apply(make_float4(a[r].x, x[r].x, a[r].y, x[r].y), h);
-    if (t0 + r < p.T) st2(p.o + (row0 + t0 + r) * p.HD + ch, h);
-    if (t0 + r == p.T - 1) *reinterpret_cast<float2*>(p.hf + (size_t)bb * p.HD + ch) = h;
+    h = apply({a[r], x[r]}, h);
+    if (r < rows) st2(o + (size_t)r * p.HD, h);
   }
+  // rows behind the end keep the state
+  if (rows > 0 && t0 + rows == p.T) *reinterpret_cast<float2*>(p.hf + (size_t)bb * p.HD + ch) = h;
 }
 
 // Tiles in the order of the reverse scan: k = 0 is the last one in time, and the
 // maps of its warps are kept from the last warp to the first.
-template <typename T, bool FROM8>
+template <typename T, bool FROM8, bool RAW>
 __global__ void __launch_bounds__(256) k_recur_bwd(const Args p) {
+  using V = typename std::conditional<FROM8, int8_t, T>::type;
   __shared__ float4 fmap[kWarps][32], rmap[kWarps][32];
   __shared__ Joint joint;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, back = kWarps - 1 - warp;
@@ -264,75 +344,91 @@ __global__ void __launch_bounds__(256) k_recur_bwd(const Args p) {
   const int groups = p.HD / kGroup, bb = at.chain / groups, cg = at.chain % groups;
   const int tile = p.tiles - 1 - at.k;
   const int ch = cg * kGroup + 2 * lane, t0 = tile * kTile + warp * kRows;
-  const size_t row0 = (size_t)bb * p.T;
+  const int rows = min(kRows, p.T - t0);
+  const size_t i0 = ((size_t)bb * p.T + t0) * p.HD + ch;
   float2 h = *reinterpret_cast<const float2*>(p.kept + ((size_t)bb * p.tiles + tile) * p.HD + ch);
-  float2 a[kRows], v[kRows], w[kRows], d[kRows], sg[kRows];
+  float2 a[kRows], v[kRows], w[kRows], d[kRows];
+  if (rows > 0) {
+    typename Raw<T>::type rg[kRows];
+    typename Raw<V>::type rv[kRows], rw[kRows];
+    float scale = 0.f;   // lane 2 r + j: of tensor j's row r
 #pragma unroll
-  for (int r = 0; r < kRows; ++r) {
-    a[r] = make_float2(1.f, 1.f);
-    v[r] = w[r] = d[r] = sg[r] = make_float2(0.f, 0.f);
-    if (t0 + r < p.T) {
-      const size_t i = (row0 + t0 + r) * p.HD + ch;
+    for (int r = 0; r < kRows; ++r) {
+      const size_t i = i0 + (size_t)min(r, rows - 1) * p.HD;
+      rv[r] = ldraw((FROM8 ? reinterpret_cast<const V*>(p.v8) : static_cast<const V*>(p.v)) + i);
+      rw[r] = ldraw((FROM8 ? reinterpret_cast<const V*>(p.w8) : static_cast<const V*>(p.w)) + i);
+      rg[r] = ldraw(static_cast<const T*>(p.g) + i);
+      d[r] = ldraw(p.dout + i);
+    }
+    if (FROM8 && lane < 2 * rows)
+      scale = (lane & 1 ? p.ws : p.vs)[(i0 - 2 * lane) / kGroup + (size_t)(lane >> 1) * groups];
+#pragma unroll
+    for (int r = 0; r < kRows; ++r) {
+      v[r] = value2(rv[r]);
+      w[r] = value2(rw[r]);
       if constexpr (FROM8) {
-        const float vs = p.vs[i / kGroup], ws = p.ws[i / kGroup];
-        v[r] = ld2(p.v8 + i);
-        w[r] = ld2(p.w8 + i);
-        v[r].x *= vs; v[r].y *= vs;
-        w[r].x *= ws; w[r].y *= ws;
-      } else {
-        v[r] = ld2(static_cast<const T*>(p.v) + i);
-        w[r] = ld2(static_cast<const T*>(p.w) + i);
+        v[r] = mul2(v[r], both(__shfl_sync(0xffffffffu, scale, 2 * r)));
+        w[r] = mul2(w[r], both(__shfl_sync(0xffffffffu, scale, 2 * r + 1)));
       }
-      sg[r] = ld2(static_cast<const T*>(p.g) + i);
-      a[r] = decay2(sg[r], p.raw);
-      w[r] = gate2(w[r], p.raw);
-      d[r] = ld2(p.dout + i);
+      w[r] = gate2<RAW>(w[r]);
+      a[r] = decay2<RAW>(value2(rg[r]));
     }
   }
-  float4 m = make_float4(1.f, 0.f, 1.f, 0.f), n = m;
+  if (rows < kRows) {   // the identity, in both directions
 #pragma unroll
-  for (int r = 0; r < kRows; ++r)
-    m = after(make_float4(a[r].x, w[r].x * v[r].x, a[r].y, w[r].y * v[r].y), m);
-#pragma unroll
-  for (int r = kRows - 1; r >= 0; --r) {
-    n.y = a[r].x * (d[r].x + n.y);
-    n.w = a[r].y * (d[r].y + n.w);
+    for (int r = 0; r < kRows; ++r)
+      if (r >= rows) a[r] = both(1.f), v[r] = w[r] = d[r] = both(0.f);
   }
-  n.x = m.x;
-  n.z = m.z;
-  fmap[warp][lane] = m;
-  rmap[back][lane] = n;
+  Map m = {a[0], mul2(w[0], v[0])}, n = identity();
+#pragma unroll
+  for (int r = 1; r < kRows; ++r) m = after({a[r], mul2(w[r], v[r])}, m);
+#pragma unroll
+  for (int r = kRows - 1; r >= 0; --r) n.b = mul2(a[r], add2(d[r], n.b));
+  n.a = m.a;
+  fmap[warp][lane] = flat(m);
+  rmap[back][lane] = flat(n);
   __syncthreads();
   float2 c = enter_tile(p, at, rmap, joint, p.dhf);
-  for (int j = 0; j < warp; ++j) h = apply(fmap[j][lane], h);
-  for (int j = 0; j < back; ++j) c = apply(rmap[j][lane], c);
+  for (int j = 0; j < warp; ++j) h = apply(unflat(fmap[j][lane]), h);
+  for (int j = 0; j < back; ++j) c = apply(unflat(rmap[j][lane]), c);
   float2 before[kRows];
 #pragma unroll
   for (int r = 0; r < kRows; ++r) {
     before[r] = h;
-    h = apply(make_float4(a[r].x, w[r].x * v[r].x, a[r].y, w[r].y * v[r].y), h);
+    h = apply({a[r], mul2(w[r], v[r])}, h);
   }
 #pragma unroll
   for (int r = kRows - 1; r >= 0; --r) {
-    const float2 dh = make_float2(d[r].x + c.x, d[r].y + c.y);
-    c = make_float2(a[r].x * dh.x, a[r].y * dh.y);
-    if (t0 + r < p.T) {
-      const size_t i = (row0 + t0 + r) * p.HD + ch;
-      float2 dw = make_float2(v[r].x * dh.x, v[r].y * dh.y);
-      float2 dg = make_float2(before[r].x * c.x, before[r].y * c.y);
-      if (p.raw) {
+    const float2 dh = add2(d[r], c);
+    c = mul2(a[r], dh);
+    if (r < rows) {
+      const size_t i = i0 + (size_t)r * p.HD;
+      float2 dw = mul2(v[r], dh), dg = mul2(before[r], c);
+      if constexpr (RAW) {
         // d sigmoid(x) = w (1 - w); dg/dx = -sigmoid(x)
-        dw.x *= w[r].x * (1.f - w[r].x);
-        dw.y *= w[r].y * (1.f - w[r].y);
-        dg.x *= -sig_from(expf(-fabsf(sg[r].x)), sg[r].x > 0.f);
-        dg.y *= -sig_from(expf(-fabsf(sg[r].y)), sg[r].y > 0.f);
+        dw = make_float2(dw.x * (w[r].x * (1.f - w[r].x)), dw.y * (w[r].y * (1.f - w[r].y)));
+        const float2 g = value2(ldraw(static_cast<const T*>(p.g) + i));   // in L2
+        dg = make_float2(-dg.x * sig(g.x), -dg.y * sig(g.y));
       }
-      st2(static_cast<T*>(p.dv) + i, make_float2(w[r].x * dh.x, w[r].y * dh.y));
+      st2(static_cast<T*>(p.dv) + i, mul2(w[r], dh));
       st2(static_cast<T*>(p.dw) + i, dw);
       st2(static_cast<T*>(p.dg) + i, dg);
     }
   }
   if (tile == 0 && warp == 0) *reinterpret_cast<float2*>(p.dh0 + (size_t)bb * p.HD + ch) = c;
+}
+
+template <bool FWD, typename T>
+void launch(const Args& p, bool int8, bool raw, cudaStream_t s) {
+  const unsigned grid = (unsigned)((size_t)p.chains * p.tiles);
+  auto go = [&](auto kernel) { kernel<<<grid, 256, 0, s>>>(p); };
+  if constexpr (FWD) {
+    if (int8) raw ? go(k_recur_fwd<T, true, true>) : go(k_recur_fwd<T, true, false>);
+    else raw ? go(k_recur_fwd<T, false, true>) : go(k_recur_fwd<T, false, false>);
+  } else {
+    if (int8) raw ? go(k_recur_bwd<T, true, true>) : go(k_recur_bwd<T, true, false>);
+    else raw ? go(k_recur_bwd<T, false, true>) : go(k_recur_bwd<T, false, false>);
+  }
 }
 
 int check(int dtype, int B, int T, int H, int D) {
@@ -401,18 +497,12 @@ extern "C" int gdn2_recur_fwd(int dtype, const void* v, const void* w, const voi
   p.v = v; p.w = w; p.g = g; p.h0 = h0; p.o = o; p.hf = h_final; p.kept = kept;
   p.v8 = static_cast<int8_t*>(v8); p.w8 = static_cast<int8_t*>(w8);
   p.vs = v_scales; p.ws = w_scales;
-  p.T = T; p.HD = H * D; p.tiles = (T + kTile - 1) / kTile; p.raw = raw;
+  p.T = T; p.HD = H * D; p.tiles = (T + kTile - 1) / kTile;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   const int e = prepare(p, B, workspace, s);
   if (e) return e;
-  const unsigned grid = (unsigned)((size_t)p.chains * p.tiles);
-  if (dtype == GDN2_F32) {
-    if (save8) k_recur_fwd<float, true><<<grid, 256, 0, s>>>(p);
-    else k_recur_fwd<float, false><<<grid, 256, 0, s>>>(p);
-  } else {
-    if (save8) k_recur_fwd<__nv_bfloat16, true><<<grid, 256, 0, s>>>(p);
-    else k_recur_fwd<__nv_bfloat16, false><<<grid, 256, 0, s>>>(p);
-  }
+  if (dtype == GDN2_F32) launch<true, float>(p, save8, raw, s);
+  else launch<true, __nv_bfloat16>(p, save8, raw, s);
   return launched();
 }
 
@@ -444,17 +534,11 @@ extern "C" int gdn2_recur_bwd(int dtype, const void* v, const void* w, const voi
   p.vs = const_cast<float*>(v_scales); p.ws = const_cast<float*>(w_scales);
   p.kept = const_cast<float*>(kept); p.dout = dout; p.dhf = dh_final;
   p.dv = dv; p.dw = dw; p.dg = dg; p.dh0 = dh0;
-  p.T = T; p.HD = H * D; p.tiles = (T + kTile - 1) / kTile; p.raw = raw;
+  p.T = T; p.HD = H * D; p.tiles = (T + kTile - 1) / kTile;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   const int e = prepare(p, B, workspace, s);
   if (e) return e;
-  const unsigned grid = (unsigned)((size_t)p.chains * p.tiles);
-  if (dtype == GDN2_F32) {
-    if (from8) k_recur_bwd<float, true><<<grid, 256, 0, s>>>(p);
-    else k_recur_bwd<float, false><<<grid, 256, 0, s>>>(p);
-  } else {
-    if (from8) k_recur_bwd<__nv_bfloat16, true><<<grid, 256, 0, s>>>(p);
-    else k_recur_bwd<__nv_bfloat16, false><<<grid, 256, 0, s>>>(p);
-  }
+  if (dtype == GDN2_F32) launch<false, float>(p, from8, raw, s);
+  else launch<false, __nv_bfloat16>(p, from8, raw, s);
   return launched();
 }
