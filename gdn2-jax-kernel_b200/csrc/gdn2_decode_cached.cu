@@ -3,14 +3,19 @@
 // it stands there), with the state read as codes, held in float32 registers
 // over the tokens of the call and stored as codes again.
 //
-// A step is bound by the state's bytes: 2 x 17 KB a head at D = 128, against
-// 2 x 64 KB for float32 states.
+// A step is bound by the state's bytes, 2 x 17 KB a head at D = 128 against
+// 2 x 64 KB for float32 states, and close behind by the instructions of taking
+// every code apart and putting it together again.
 //
-// One CTA per (row, head).  A thread holds 8 columns (one 8-byte load of codes)
-// of R key rows; the D / 8 lanes of a row sit in one warp, so the maximum of a
-// group of 64 columns takes three shuffles.  The two products with the state
-// (W^T h and qg^T h) are summed over a thread's rows, over the row lanes of the
-// warp, then over the warps in shared memory, always in the same order.
+// One CTA per (row, head).  The head's codes and scales (17 KB, contiguous) come
+// to shared memory by asynchronous copies, so the bytes in flight do not cost
+// registers and five CTAs fit an SM.  A thread works on 8 columns (one 8-byte
+// word of codes) of R key rows; the D / 8 lanes of a row sit in one warp, so the
+// maximum of a group of 64 columns takes three shuffles.  The two products with
+// the state (W^T h and qg^T h) are summed over a thread's rows, over the row
+// lanes of the warp, then over the warps in shared memory, always in the same
+// order.  A call of one token takes the codes apart twice (for the products and
+// for the update); a call of more tokens keeps float32 values in registers.
 #include "../../include/gdn2.h"
 #include "gdn2_int8.cuh"
 
@@ -19,139 +24,250 @@ int report_error(int code, const char* msg);
 
 namespace {
 
-template <typename T, int D>
-__global__ void __launch_bounds__(256)
+template <int D> struct Shape {
+  static constexpr int NW = D / 16;          // warps
+  static constexpr int CL = D / 8;           // lanes of a row
+  static constexpr int RW = 32 / CL;         // rows of a warp's load
+  static constexpr int R = D / (NW * RW);    // rows of a thread
+  static_assert(R % 4 == 0, "scales leave by fours");
+  static constexpr int G = D / kGroup;
+};
+
+// 16 bytes to shared memory, asynchronously.
+__device__ __forceinline__ void copy16(void* to, const void* from) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;"
+               ::"r"((unsigned)__cvta_generic_to_shared(to)), "l"(from) : "memory");
+}
+__device__ __forceinline__ void copies_done() { asm volatile("cp.async.wait_all;" ::: "memory"); }
+
+// The 8 codes of a row as float32 pairs.
+__device__ __forceinline__ void codes8(uint2 c, float2 (&f)[4]) {
+  f[0] = make_float2(code_f<0>(c.x), code_f<1>(c.x));
+  f[1] = make_float2(code_f<2>(c.x), code_f<3>(c.x));
+  f[2] = make_float2(code_f<0>(c.y), code_f<1>(c.y));
+  f[3] = make_float2(code_f<2>(c.y), code_f<3>(c.y));
+}
+__device__ __forceinline__ float top8(const float2 (&s)[4]) {
+  return max_abs3(max_abs3(max_abs3(fabsf(s[0].x), s[0].y, s[1].x), s[1].y, s[2].x),
+                  max_abs(s[2].y, s[3].x), s[3].y);
+}
+
+template <typename T, int D, bool ONE>
+__global__ void __launch_bounds__(Shape<D>::NW * 32, D == 64 ? (ONE ? 8 : 6) : ONE ? 5 : 2)
 k_decode_cached(const T* __restrict__ q, const T* __restrict__ k, const T* __restrict__ v,
                 const T* __restrict__ w, const T* __restrict__ b, const T* __restrict__ g,
                 int8_t* codes, float* scales, const int* __restrict__ src,
                 const int* __restrict__ dst, float* __restrict__ o, int B, int T_, int H, int S,
                 float scale, float clip, int gates) {
-  constexpr int NW = 8, CL = D / 8, RW = 32 / CL, R = D / (NW * RW), G = D / kGroup;
-  __shared__ float4 vec[D];            // W, qg, kg, e^{gc_last} of a token
-  __shared__ float2 part[NW][D];       // per warp: W^T h, qg^T h
-  __shared__ float red[D / 32], su[D], snew[D];
+  constexpr int NW = Shape<D>::NW, CL = Shape<D>::CL, RW = Shape<D>::RW, R = Shape<D>::R,
+                G = Shape<D>::G;
+  __shared__ __align__(16) int8_t scodes[D * D];
+  __shared__ __align__(16) float sscales[D * G];
+  __shared__ float4 vec[ONE ? 1 : 2][D];   // W, qg, kg, e^{gc_last} of a token
+  __shared__ float red[ONE ? 1 : 2][D / 32], su[ONE ? 1 : 2][D];
+  __shared__ __align__(16) float2 part[NW][D];   // per warp: W^T h, qg^T h
+  __shared__ __align__(16) float snew[D];
   const int h = blockIdx.x, bb = blockIdx.y, tid = threadIdx.x;
   const int lane = tid & 31, warp = tid >> 5, cl = lane % CL, rl = lane / CL;
+  const float a1 = san(1.f, clip);   // A = (I + Akk)^-1 of a one-token chunk, sanitised
+
+  const int from = src ? src[bb] : bb, to = dst ? dst[bb] : bb;
+  const bool some = from >= 0 && from < S;
+  if (some) {
+    const size_t at = ((size_t)from * H + h) * D;
+    const int8_t* c = codes + at * D;
+    const float* z = scales + at * G;
+#pragma unroll
+    for (int i = 0; i < D * D / (NW * 32 * 16); ++i)
+      copy16(scodes + (i * NW * 32 + tid) * 16, c + (i * NW * 32 + tid) * 16);
+    if (tid < D * G / 4) copy16(sscales + tid * 4, z + tid * 4);
+  }
+
+  // a token's vectors, by the first D threads: loaded, then put to shared memory
+  float tq, tk, tv, tw, tb, tg;
+  auto load = [&](size_t off) {
+    tq = to_f<T>(q[off + tid]);
+    tk = to_f<T>(k[off + tid]);
+    tv = to_f<T>(v[off + tid]);
+    tw = to_f<T>(w[off + tid]);
+    tb = to_f<T>(b[off + tid]);
+    tg = to_f<T>(g[off + tid]);
+  };
+  auto put = [&](int buf) {
+    if (gates) {
+      tw = gate_act(tw, kGateW);
+      tb = gate_act(tb, kGateB);
+      tg = gate_act(tg, kGateG);
+    }
+    const float eg = expf(tg);
+    vec[buf][tid] = make_float4(san(a1 * (tb * tk * eg), clip), san(tq * eg, clip), san(tk, clip),
+                                expf(san(tg, clip)));
+    su[buf][tid] = san(a1 * (tw * tv), clip);
+    float qk = tq * tk;
+#pragma unroll
+    for (int x = 16; x; x >>= 1) qk += __shfl_xor_sync(0xffffffffu, qk, x);
+    if (lane == 0) red[buf][warp] = qk;
+  };
+  size_t off = ((size_t)bb * T_ * H + h) * D;
+  if (tid < D) {
+    load(off);
+    put(0);
+  }
 
   // A destination that is another row's source or destination would make the
   // result depend on which block runs first; such a row, and one whose slots
   // lie outside the cache, gets NaN outputs and no state is written for it.
-  const int from = src ? src[bb] : bb, to = dst ? dst[bb] : bb;
   int bad = from < -1 || from >= S || to < -1 || to >= S;
   if (to >= 0)
-    for (int j = tid; j < B; j += 256)
+    for (int j = tid; j < B; j += NW * 32)
       if (j != bb) {
         if (src) bad |= src[j] == to;
         if (dst != src) bad |= dst[j] == to;
       }
+  copies_done();
   bad = __syncthreads_or(bad);
   if (bad) {
-    for (int t = 0; t < T_; ++t)
-      if (tid < D) o[(((size_t)bb * T_ + t) * H + h) * D + tid] = __uint_as_float(0x7fc00000u);
+    for (int t = 0; t < T_; ++t, off += (size_t)H * D)
+      if (tid < D) o[off + tid] = __uint_as_float(0x7fc00000u);
     return;
   }
 
-  float s[R][8];
-#pragma unroll
-  for (int r = 0; r < R; ++r) {
-    const int row = (r * NW + warp) * RW + rl;
-    uint2 c = make_uint2(0, 0);
-    float sc = 0.f;
-    if (from >= 0) {
-      const size_t at = (((size_t)from * H + h) * D + row);
-      c = *reinterpret_cast<const uint2*>(codes + at * D + cl * 8);
-      sc = scales[at * G + cl * 8 / kGroup];
-    }
-    if (!(fabsf(sc) <= 3.4e38f)) sc = 0.f;   // the sanitiser's NaN -> 0
-    const unsigned lo = c.x ^ 0x80808080u, hi = c.y ^ 0x80808080u;
-    s[r][0] = code_f<0>(lo) * sc; s[r][1] = code_f<1>(lo) * sc;
-    s[r][2] = code_f<2>(lo) * sc; s[r][3] = code_f<3>(lo) * sc;
-    s[r][4] = code_f<0>(hi) * sc; s[r][5] = code_f<1>(hi) * sc;
-    s[r][6] = code_f<2>(hi) * sc; s[r][7] = code_f<3>(hi) * sc;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) s[r][i] = san(s[r][i], clip);
-  }
+  // row r of this thread: its scale (0 for a scale that is not finite and for the
+  // zero state, where the codes are whatever the memory holds) and its codes
+  auto row_of = [&](int r) { return (r * NW + warp) * RW + rl; };
+  auto scale_of = [&](int row) {
+    const float z = sscales[row * G + cl * 8 / kGroup];
+    return some && fabsf(z) <= 3.402823466e38f ? z : 0.f;
+  };
+  auto codes_of = [&](int row, float2 (&f)[4]) {
+    uint2 c = *reinterpret_cast<const uint2*>(scodes + row * D + cl * 8);
+    c.x ^= 0x80808080u;
+    c.y ^= 0x80808080u;
+    codes8(c, f);
+  };
 
-  const float a1 = san(1.f, clip);   // A = (I + Akk)^-1 of a one-token chunk, sanitised
-  for (int t = 0; t < T_; ++t) {
-    const size_t off = (((size_t)bb * T_ + t) * H + h) * D;
-    if (tid < D) {
-      const float qv = to_f<T>(q[off + tid]), kv = to_f<T>(k[off + tid]);
-      const float gv = ld_gate<T>(g + off + tid, gates, kGateG), eg = expf(gv);
-      vec[tid] = make_float4(
-          san(a1 * (ld_gate<T>(b + off + tid, gates, kGateB) * kv * eg), clip),
-          san(qv * eg, clip), san(kv, clip), expf(san(gv, clip)));
-      su[tid] = san(a1 * (ld_gate<T>(w + off + tid, gates, kGateW) * to_f<T>(v[off + tid])), clip);
-      float qk = qv * kv;
-#pragma unroll
-      for (int x = 16; x; x >>= 1) qk += __shfl_xor_sync(0xffffffffu, qk, x);
-      if (lane == 0) red[warp] = qk;
-    }
-    __syncthreads();
-    float a[8] = {}, c[8] = {};
+  float2 s[ONE ? 1 : R][4];
+  if constexpr (!ONE) {
 #pragma unroll
     for (int r = 0; r < R; ++r) {
-      const float4 z = vec[(r * NW + warp) * RW + rl];
+      const float z = scale_of(row_of(r));
+      codes_of(row_of(r), s[r]);
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        a[i] = fmaf(z.x, s[r][i], a[i]);
-        c[i] = fmaf(z.y, s[r][i], c[i]);
+      for (int i = 0; i < 4; ++i) s[r][i] = mul2(s[r][i], both(z));
+    }
+  }
+
+  for (int t = 0; t < (ONE ? 1 : T_); ++t, off += (size_t)H * D) {
+    const int buf = ONE ? 0 : t & 1;
+    const bool more = !ONE && t + 1 < T_ && tid < D;
+    if (more) load(off + (size_t)H * D);
+    float2 wa[4] = {}, qa[4] = {};
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      float4 z = vec[buf][row_of(r)];
+      if constexpr (ONE) {
+        const float x = scale_of(row_of(r));
+        codes_of(row_of(r), s[0]);
+        z.x *= x;
+        z.y *= x;
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        wa[i] = fma2(both(z.x), s[ONE ? 0 : r][i], wa[i]);
+        qa[i] = fma2(both(z.y), s[ONE ? 0 : r][i], qa[i]);
       }
     }
 #pragma unroll
     for (int x = CL; x < 32; x <<= 1)
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        a[i] += __shfl_xor_sync(0xffffffffu, a[i], x);
-        c[i] += __shfl_xor_sync(0xffffffffu, c[i], x);
+      for (int i = 0; i < 4; ++i) {
+        wa[i].x += __shfl_xor_sync(0xffffffffu, wa[i].x, x);
+        wa[i].y += __shfl_xor_sync(0xffffffffu, wa[i].y, x);
+        qa[i].x += __shfl_xor_sync(0xffffffffu, qa[i].x, x);
+        qa[i].y += __shfl_xor_sync(0xffffffffu, qa[i].y, x);
       }
     if (rl == 0)
 #pragma unroll
-      for (int i = 0; i < 8; ++i) part[warp][cl * 8 + i] = make_float2(a[i], c[i]);
+      for (int i = 0; i < 4; ++i)
+        *reinterpret_cast<float4*>(&part[warp][cl * 8 + 2 * i]) =
+            make_float4(wa[i].x, qa[i].x, wa[i].y, qa[i].y);
+    if (more) put(buf ^ 1);
     __syncthreads();
     if (tid < D) {
       float dot = 0.f, wh = 0.f, qh = 0.f;
 #pragma unroll
-      for (int i = 0; i < D / 32; ++i) dot += red[i];
+      for (int i = 0; i < D / 32; ++i) dot += red[buf][i];
 #pragma unroll
       for (int i = 0; i < NW; ++i) {
         const float2 p = part[i][tid];
         wh += p.x;
         qh += p.y;
       }
-      const float vn = su[tid] - wh;
+      const float vn = su[buf][tid] - wh;
       snew[tid] = vn;
       o[off + tid] = san(scale * qh + san(scale * dot, clip) * vn, clip);
     }
     __syncthreads();
-    float vn[8];
+    if constexpr (!ONE) {
+      float2 vn[4];
+      *reinterpret_cast<float4*>(vn) = *reinterpret_cast<const float4*>(snew + cl * 8);
+      *reinterpret_cast<float4*>(vn + 2) = *reinterpret_cast<const float4*>(snew + cl * 8 + 4);
+      float top = 0.f;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) vn[i] = snew[cl * 8 + i];
+      for (int r = 0; r < R; ++r) {
+        const float4 z = vec[buf][row_of(r)];
 #pragma unroll
-    for (int r = 0; r < R; ++r) {
-      const float4 z = vec[(r * NW + warp) * RW + rl];
+        for (int i = 0; i < 4; ++i) s[r][i] = fma2(both(z.w), s[r][i], mul2(both(z.z), vn[i]));
+        top = max_abs(top, top8(s[r]));
+      }
+      if (!(top <= clip))   // seldom: the sanitiser acts
 #pragma unroll
-      for (int i = 0; i < 8; ++i) s[r][i] = san(fmaf(z.w, s[r][i], z.z * vn[i]), clip);
+        for (int r = 0; r < R; ++r)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) s[r][i] = make_float2(san(s[r][i].x, clip), san(s[r][i].y, clip));
     }
-    __syncthreads();   // the token vectors are rewritten
   }
 
   if (to < 0) return;
+  float2 vn[4];
+  *reinterpret_cast<float4*>(vn) = *reinterpret_cast<const float4*>(snew + cl * 8);
+  *reinterpret_cast<float4*>(vn + 2) = *reinterpret_cast<const float4*>(snew + cl * 8 + 4);
+  const size_t row0 = ((size_t)to * H + h) * D;
+  float mine = 0.f;   // of row (lane & 3) of four: lanes share the scales' divisions
 #pragma unroll
   for (int r = 0; r < R; ++r) {
-    float top = fabsf(s[r][0]);
+    const int row = row_of(r);
+    float2 (&x)[4] = s[ONE ? 0 : r];
+    if constexpr (ONE) {
+      const float4 z = vec[0][row];
+      const float y = scale_of(row);
+      codes_of(row, x);
 #pragma unroll
-    for (int i = 1; i < 8; ++i) top = max_abs(top, s[r][i]);
+      for (int i = 0; i < 4; ++i) x[i] = fma2(both(z.w * y), x[i], mul2(both(z.z), vn[i]));
+    }
+    float top = top8(x);
 #pragma unroll
-    for (int x = 1; x < 8; x <<= 1) top = max_abs(top, __shfl_xor_sync(0xffffffffu, top, x));
+    for (int y = 1; y < 8; y <<= 1) top = max_abs(top, __shfl_xor_sync(0xffffffffu, top, y));
+    if (ONE && __any_sync(0xffffffffu, !(top <= clip))) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) x[i] = make_float2(san(x[i].x, clip), san(x[i].y, clip));
+      top = top8(x);
+#pragma unroll
+      for (int y = 1; y < 8; y <<= 1) top = max_abs(top, __shfl_xor_sync(0xffffffffu, top, y));
+    }
+    // the nearest code by float32 arithmetic alone: the value carries rounding
+    // errors of its own, 2.2e-5 of a step more do not matter
     const float inv = group_inv(top);
-    uint2 c;
-    auto code = [&](int i) { return int8_code_near(s[r][i], inv); };
-    c.x = pack4(code(0), code(1), code(2), code(3));
-    c.y = pack4(code(4), code(5), code(6), code(7));
-    const size_t at = (((size_t)to * H + h) * D + (r * NW + warp) * RW + rl);
-    *reinterpret_cast<uint2*>(codes + at * D + cl * 8) = c;
-    if (cl % 8 == 0) scales[at * G + cl * 8 / kGroup] = group_scale(top);
+    float2 n[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) n[i] = fma2(x[i], both(inv), both(kCodeBias));
+    auto u = [](float y) { return __float_as_uint(y); };
+    *reinterpret_cast<uint2*>(codes + (row0 + row) * D + cl * 8) =
+        make_uint2(pack4(u(n[0].x), u(n[0].y), u(n[1].x), u(n[1].y)),
+                   pack4(u(n[2].x), u(n[2].y), u(n[3].x), u(n[3].y)));
+    if ((cl & 3) == (r & 3)) mine = top;
+    if ((r & 3) == 3 && cl % 8 < 4)
+      scales[(row0 + row_of(r - 3 + (cl & 3))) * G + cl * 8 / kGroup] = group_scale(mine);
   }
 }
 
@@ -160,9 +276,12 @@ void launch(const void* q, const void* k, const void* v, const void* w, const vo
             const void* g, void* codes, float* scales, const int* src, const int* dst, float* o,
             int B, int T_, int H, int S, float scale, float clip, int gates, cudaStream_t s) {
   auto c = [](const void* x) { return static_cast<const T*>(x); };
-  k_decode_cached<T, D><<<dim3(H, B), 256, 0, s>>>(c(q), c(k), c(v), c(w), c(b), c(g),
-                                                   static_cast<int8_t*>(codes), scales, src, dst,
-                                                   o, B, T_, H, S, scale, clip, gates);
+  auto go = [&](auto kernel) {
+    kernel<<<dim3(H, B), Shape<D>::NW * 32, 0, s>>>(c(q), c(k), c(v), c(w), c(b), c(g),
+                                                    static_cast<int8_t*>(codes), scales, src, dst,
+                                                    o, B, T_, H, S, scale, clip, gates);
+  };
+  T_ == 1 ? go(k_decode_cached<T, D, true>) : go(k_decode_cached<T, D, false>);
 }
 
 }  // namespace
@@ -187,8 +306,8 @@ extern "C" int gdn2_decode_cached(int dtype, const void* q, const void* k, const
     return report_error(GDN2_ERR_INVALID, "gdn2_decode_cached: clip must be positive, scale finite");
   if (!q || !k || !v || !w || !b || !g || !o || !codes || !scales)
     return report_error(GDN2_ERR_INVALID, "gdn2_decode_cached: null buffer pointer");
-  if ((reinterpret_cast<uintptr_t>(codes) & 15) || (reinterpret_cast<uintptr_t>(scales) & 3))
-    return report_error(GDN2_ERR_INVALID, "gdn2_decode_cached: codes must be 16-byte aligned");
+  if ((reinterpret_cast<uintptr_t>(codes) & 15) || (reinterpret_cast<uintptr_t>(scales) & 15))
+    return report_error(GDN2_ERR_INVALID, "gdn2_decode_cached: codes and scales must be 16-byte aligned");
   if ((!src || !dst) && B > S)
     return report_error(GDN2_ERR_INVALID, "gdn2_decode_cached: more rows than slots");
   if (!src != !dst)

@@ -20,6 +20,8 @@ namespace gdn2 {
 
 constexpr int kGroup = 64;            // values that share a scale
 constexpr float kInt8Tiny = 0x1p-100f;
+// 1.5 * 2^23: added to |y| < 2^22 it leaves rint(y) in the low bits
+constexpr float kCodeBias = 12582912.f;
 
 // |x| as an ordered integer: NaN above infinity above every finite value, so
 // an integer maximum keeps NaN (a float maximum would drop it).
@@ -29,6 +31,40 @@ __device__ __forceinline__ unsigned abs_bits(float x) { return __float_as_uint(x
 __device__ __forceinline__ float max_abs(float x, float y) {
   float r;
   asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(fabsf(x)), "f"(fabsf(y)));
+  return r;
+}
+
+// Two values as one operand of the packed float32 instructions.
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+  float2 d;
+  asm("{.reg .b64 x, y, z;\n\t"
+      "mov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\tmov.b64 z, {%6, %7};\n\t"
+      "fma.rn.f32x2 x, x, y, z;\n\tmov.b64 {%0, %1}, x;}"
+      : "=f"(d.x), "=f"(d.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+  return d;
+}
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+  float2 d;
+  asm("{.reg .b64 x, y;\n\t"
+      "mov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\t"
+      "mul.rn.f32x2 x, x, y;\n\tmov.b64 {%0, %1}, x;}"
+      : "=f"(d.x), "=f"(d.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return d;
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+  float2 d;
+  asm("{.reg .b64 x, y;\n\t"
+      "mov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\t"
+      "add.rn.f32x2 x, x, y;\n\tmov.b64 {%0, %1}, x;}"
+      : "=f"(d.x), "=f"(d.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return d;
+}
+__device__ __forceinline__ float2 both(float x) { return make_float2(x, x); }
+
+// max|.| of three values; NaN stays.
+__device__ __forceinline__ float max_abs3(float x, float y, float z) {
+  float r;
+  asm("max.NaN.abs.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(x), "f"(y), "f"(z));
   return r;
 }
 
@@ -53,7 +89,7 @@ static __device__ __noinline__ float int8_border(float x, float y, float top) {
   return copysignf(lo + (up ? 1.f : 0.f), x);
 }
 // The codes of N values of one group, each in the low byte of a word.
-// 1.5 * 2^23 added to |y| <= 127.01 rounds y = x * inv to a whole number, in the
+// kCodeBias added to y = x * inv, |y| <= 127.01, rounds it to a whole number in the
 // low bits (the conversion and rounding instructions run at an eighth of the
 // rate).  y is off by at most 127 * 2^-22.5 = 2.2e-5, so only a y within 1e-4 of
 // a half can round the wrong way: one value in 5000 is decided in float64.
@@ -63,23 +99,18 @@ __device__ __forceinline__ void int8_codes(const float (&x)[N], float inv, float
   float far = 0.f;
 #pragma unroll
   for (int i = 0; i < N; ++i) {
-    const float t = fmaf(x[i], inv, 12582912.f);
-    far = fmaxf(far, fabsf(fmaf(x[i], inv, 12582912.f - t)));
+    const float t = fmaf(x[i], inv, kCodeBias);
+    far = fmaxf(far, fabsf(fmaf(x[i], inv, kCodeBias - t)));
     code[i] = __float_as_uint(t);
   }
   if (far > 0.4999f) {
 #pragma unroll
     for (int i = 0; i < N; ++i) {
-      const float y = x[i] * inv, r = __uint_as_float(code[i]) - 12582912.f;
+      const float y = x[i] * inv, r = __uint_as_float(code[i]) - kCodeBias;
       if (fabsf(y - r) > 0.4998f)
-        code[i] = __float_as_uint(int8_border(x[i], y, top) + 12582912.f);
+        code[i] = __float_as_uint(int8_border(x[i], y, top) + kCodeBias);
     }
   }
-}
-// The nearest code by float32 arithmetic alone, for values that carry rounding
-// errors of their own: off from a half step by at most 2.2e-5 of a step.
-__device__ __forceinline__ unsigned int8_code_near(float x, float inv) {
-  return __float_as_uint(fmaf(x, inv, 12582912.f));
 }
 __device__ __forceinline__ unsigned pack4(unsigned a, unsigned b, unsigned c, unsigned d) {
   return __byte_perm(__byte_perm(a, b, 0x0040), __byte_perm(c, d, 0x0040), 0x5410);

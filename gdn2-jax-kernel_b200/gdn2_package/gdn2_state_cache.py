@@ -51,8 +51,9 @@ class Gdn2StateCache:
         if tuple(scales.shape) != want or scales.dtype != torch.float32 \
                 or scales.device != codes.device:
             raise _fwd.Gdn2ShapeError(f"scales must be {want} float32 on the codes' device")
-        if not codes.is_contiguous() or not scales.is_contiguous() or codes.data_ptr() % 16:
-            raise _fwd.Gdn2ShapeError("codes and scales must be contiguous, codes 16-byte aligned")
+        if not codes.is_contiguous() or not scales.is_contiguous() or codes.data_ptr() % 16 \
+                or scales.data_ptr() % 16:
+            raise _fwd.Gdn2ShapeError("codes and scales must be contiguous and 16-byte aligned")
         self = cls.__new__(cls)
         self.codes, self.scales = codes, scales
         return self

@@ -57,7 +57,7 @@ def test_state_entry_points_refuse():
 
     for kw in (dict(dtype=3), dict(q=None), dict(codes=None), dict(scales=None), dict(o=None),
                dict(B=0), dict(T=0), dict(H=0), dict(S=0), dict(D=256), dict(clip=-1.0),
-               dict(scale=float("nan")), dict(codes=ODD), dict(src=None), dict(dst=None),
+               dict(scale=float("nan")), dict(codes=ODD), dict(scales=ODD), dict(src=None), dict(dst=None),
                dict(src=None, dst=None, B=3), dict(B=65536)):
         assert decode(**kw) == bad, kw
 
