@@ -24,6 +24,9 @@ int report_error(int code, const char* msg);
 
 namespace {
 
+#ifndef MINB
+#define MINB 3
+#endif
 template <int D> struct Shape {
   static constexpr int NW = D / 16;          // warps
   static constexpr int CL = D / 8;           // lanes of a row
@@ -40,20 +43,37 @@ __device__ __forceinline__ void copy16(void* to, const void* from) {
 }
 __device__ __forceinline__ void copies_done() { asm volatile("cp.async.wait_all;" ::: "memory"); }
 
-// The 8 codes of a row as float32 pairs.
+// The 8 codes of a row as float32 pairs: by byte moves and packed additions, or
+// by the conversion unit, which is idle otherwise (an eighth of the rate, one
+// instruction instead of one and a half).
 __device__ __forceinline__ void codes8(uint2 c, float2 (&f)[4]) {
-  f[0] = make_float2(code_f<0>(c.x), code_f<1>(c.x));
-  f[1] = make_float2(code_f<2>(c.x), code_f<3>(c.x));
-  f[2] = make_float2(code_f<0>(c.y), code_f<1>(c.y));
-  f[3] = make_float2(code_f<2>(c.y), code_f<3>(c.y));
+  const unsigned x = c.x ^ 0x80808080u, y = c.y ^ 0x80808080u;
+  const float2 bias = both(-8388736.f);
+  f[0] = add2(make_float2(biased_f<0>(x), biased_f<1>(x)), bias);
+  f[1] = add2(make_float2(biased_f<2>(x), biased_f<3>(x)), bias);
+  f[2] = add2(make_float2(biased_f<0>(y), biased_f<1>(y)), bias);
+  f[3] = add2(make_float2(biased_f<2>(y), biased_f<3>(y)), bias);
+}
+__device__ __forceinline__ void convert8(uint2 c, float2 (&f)[4]) {
+  auto at = [](unsigned x, int i) { return (float)(int8_t)(x >> 8 * i); };
+  f[0] = make_float2(at(c.x, 0), at(c.x, 1));
+  f[1] = make_float2(at(c.x, 2), at(c.x, 3));
+  f[2] = make_float2(at(c.y, 0), at(c.y, 1));
+  f[3] = make_float2(at(c.y, 2), at(c.y, 3));
 }
 __device__ __forceinline__ float top8(const float2 (&s)[4]) {
   return max_abs3(max_abs3(max_abs3(fabsf(s[0].x), s[0].y, s[1].x), s[1].y, s[2].x),
                   max_abs(s[2].y, s[3].x), s[3].y);
 }
 
+// h <- d h + kg vn on 8 columns.
+__device__ __forceinline__ void update8(float2 (&x)[4], float d, float kg, const float2 (&vn)[4]) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) x[i] = fma2(both(d), x[i], mul2(both(kg), vn[i]));
+}
+
 template <typename T, int D, bool ONE>
-__global__ void __launch_bounds__(Shape<D>::NW * 32, D == 64 ? (ONE ? 8 : 6) : ONE ? 5 : 2)
+__global__ void __launch_bounds__(Shape<D>::NW * 32, D == 64 ? 6 : ONE ? MINB : 2)
 k_decode_cached(const T* __restrict__ q, const T* __restrict__ k, const T* __restrict__ v,
                 const T* __restrict__ w, const T* __restrict__ b, const T* __restrict__ g,
                 int8_t* codes, float* scales, const int* __restrict__ src,
@@ -81,6 +101,8 @@ k_decode_cached(const T* __restrict__ q, const T* __restrict__ k, const T* __res
     for (int i = 0; i < D * D / (NW * 32 * 16); ++i)
       copy16(scodes + (i * NW * 32 + tid) * 16, c + (i * NW * 32 + tid) * 16);
     if (tid < D * G / 4) copy16(sscales + tid * 4, z + tid * 4);
+  } else {   // the zero state: scales of 0 beside codes of any value
+    for (int i = tid; i < D * G; i += NW * 32) sscales[i] = 0.f;
   }
 
   // a token's vectors, by the first D threads: loaded, then put to shared memory
@@ -132,26 +154,17 @@ k_decode_cached(const T* __restrict__ q, const T* __restrict__ k, const T* __res
     return;
   }
 
-  // row r of this thread: its scale (0 for a scale that is not finite and for the
-  // zero state, where the codes are whatever the memory holds) and its codes
+  // row r of this thread, its scale (NaN as 0) and its codes
   auto row_of = [&](int r) { return (r * NW + warp) * RW + rl; };
-  auto scale_of = [&](int row) {
-    const float z = sscales[row * G + cl * 8 / kGroup];
-    return some && fabsf(z) <= 3.402823466e38f ? z : 0.f;
-  };
-  auto codes_of = [&](int row, float2 (&f)[4]) {
-    uint2 c = *reinterpret_cast<const uint2*>(scodes + row * D + cl * 8);
-    c.x ^= 0x80808080u;
-    c.y ^= 0x80808080u;
-    codes8(c, f);
-  };
+  auto scale_of = [&](int row) { return fmaxf(sscales[row * G + cl * 8 / kGroup], 0.f); };
+  auto word_of = [&](int row) { return *reinterpret_cast<const uint2*>(scodes + row * D + cl * 8); };
 
-  float2 s[ONE ? 1 : R][4];
+  float2 s[ONE ? 4 : R][4];
   if constexpr (!ONE) {
 #pragma unroll
     for (int r = 0; r < R; ++r) {
       const float z = scale_of(row_of(r));
-      codes_of(row_of(r), s[r]);
+      codes8(word_of(row_of(r)), s[r]);
 #pragma unroll
       for (int i = 0; i < 4; ++i) s[r][i] = mul2(s[r][i], both(z));
     }
@@ -167,14 +180,14 @@ k_decode_cached(const T* __restrict__ q, const T* __restrict__ k, const T* __res
       float4 z = vec[buf][row_of(r)];
       if constexpr (ONE) {
         const float x = scale_of(row_of(r));
-        codes_of(row_of(r), s[0]);
+        convert8(word_of(row_of(r)), s[r & 3]);
         z.x *= x;
         z.y *= x;
       }
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        wa[i] = fma2(both(z.x), s[ONE ? 0 : r][i], wa[i]);
-        qa[i] = fma2(both(z.y), s[ONE ? 0 : r][i], qa[i]);
+        wa[i] = fma2(both(z.x), s[ONE ? r & 3 : r][i], wa[i]);
+        qa[i] = fma2(both(z.y), s[ONE ? r & 3 : r][i], qa[i]);
       }
     }
 #pragma unroll
@@ -216,8 +229,7 @@ k_decode_cached(const T* __restrict__ q, const T* __restrict__ k, const T* __res
 #pragma unroll
       for (int r = 0; r < R; ++r) {
         const float4 z = vec[buf][row_of(r)];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) s[r][i] = fma2(both(z.w), s[r][i], mul2(both(z.z), vn[i]));
+        update8(s[r], z.w, z.z, vn);
         top = max_abs(top, top8(s[r]));
       }
       if (!(top <= clip))   // seldom: the sanitiser acts
@@ -233,41 +245,59 @@ k_decode_cached(const T* __restrict__ q, const T* __restrict__ k, const T* __res
   *reinterpret_cast<float4*>(vn) = *reinterpret_cast<const float4*>(snew + cl * 8);
   *reinterpret_cast<float4*>(vn + 2) = *reinterpret_cast<const float4*>(snew + cl * 8 + 4);
   const size_t row0 = ((size_t)to * H + h) * D;
-  float mine = 0.f;   // of row (lane & 3) of four: lanes share the scales' divisions
+  // Four rows at a time: the maxima of the four are passed around the 8 lanes of a
+  // group so that each lane ends with one row's, works out that row's scale, and
+  // hands 127 / max back.
+  const int own = cl & 3;
 #pragma unroll
-  for (int r = 0; r < R; ++r) {
-    const int row = row_of(r);
-    float2 (&x)[4] = s[ONE ? 0 : r];
-    if constexpr (ONE) {
-      const float4 z = vec[0][row];
-      const float y = scale_of(row);
-      codes_of(row, x);
+  for (int r0 = 0; r0 < R; r0 += 4) {
+    float2 (&x)[4][4] = *reinterpret_cast<float2 (*)[4][4]>(&s[ONE ? 0 : r0]);
+    float top[4];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) x[i] = fma2(both(z.w * y), x[i], mul2(both(z.z), vn[i]));
+    for (int j = 0; j < 4; ++j) {
+      if constexpr (ONE) {
+        const int row = row_of(r0 + j);
+        const float4 z = vec[0][row];
+        codes8(word_of(row), x[j]);
+        update8(x[j], z.w * scale_of(row), z.z, vn);
+      }
+      top[j] = top8(x[j]);
     }
-    float top = top8(x);
+    auto around = [&] {
+      const bool hi = own & 2, odd = own & 1;
+      float t0 = hi ? top[2] : top[0], t1 = hi ? top[3] : top[1];
+      const float u0 = hi ? top[0] : top[2], u1 = hi ? top[1] : top[3];
+      t0 = max_abs(t0, __shfl_xor_sync(0xffffffffu, u0, 2));
+      t1 = max_abs(t1, __shfl_xor_sync(0xffffffffu, u1, 2));
+      float m = odd ? t1 : t0;
+      m = max_abs(m, __shfl_xor_sync(0xffffffffu, odd ? t0 : t1, 1));
+      return max_abs(m, __shfl_xor_sync(0xffffffffu, m, 4));
+    };
+    float m = around();   // of row r0 + own
+    if (ONE && __any_sync(0xffffffffu, !(m <= clip))) {   // seldom: the sanitiser acts
 #pragma unroll
-    for (int y = 1; y < 8; y <<= 1) top = max_abs(top, __shfl_xor_sync(0xffffffffu, top, y));
-    if (ONE && __any_sync(0xffffffffu, !(top <= clip))) {
+      for (int j = 0; j < 4; ++j) {
 #pragma unroll
-      for (int i = 0; i < 4; ++i) x[i] = make_float2(san(x[i].x, clip), san(x[i].y, clip));
-      top = top8(x);
-#pragma unroll
-      for (int y = 1; y < 8; y <<= 1) top = max_abs(top, __shfl_xor_sync(0xffffffffu, top, y));
+        for (int i = 0; i < 4; ++i) x[j][i] = make_float2(san(x[j][i].x, clip), san(x[j][i].y, clip));
+        top[j] = top8(x[j]);
+      }
+      m = around();
     }
-    // the nearest code by float32 arithmetic alone: the value carries rounding
-    // errors of its own, 2.2e-5 of a step more do not matter
-    const float inv = group_inv(top);
-    float2 n[4];
+    if (cl % 8 < 4) scales[(row0 + row_of(r0 + own)) * G + cl * 8 / kGroup] = group_scale(m);
+    const float inv = group_inv(m);
 #pragma unroll
-    for (int i = 0; i < 4; ++i) n[i] = fma2(x[i], both(inv), both(kCodeBias));
-    auto u = [](float y) { return __float_as_uint(y); };
-    *reinterpret_cast<uint2*>(codes + (row0 + row) * D + cl * 8) =
-        make_uint2(pack4(u(n[0].x), u(n[0].y), u(n[1].x), u(n[1].y)),
-                   pack4(u(n[2].x), u(n[2].y), u(n[3].x), u(n[3].y)));
-    if ((cl & 3) == (r & 3)) mine = top;
-    if ((r & 3) == 3 && cl % 8 < 4)
-      scales[(row0 + row_of(r - 3 + (cl & 3))) * G + cl * 8 / kGroup] = group_scale(mine);
+    for (int j = 0; j < 4; ++j) {
+      // the nearest code by float32 arithmetic alone: the value carries rounding
+      // errors of its own, 2.2e-5 of a step more do not matter
+      const float y = __shfl_sync(0xffffffffu, inv, (lane & ~3) | j);
+      float2 n[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) n[i] = fma2(x[j][i], both(y), both(kCodeBias));
+      auto u = [](float f) { return __float_as_uint(f); };
+      *reinterpret_cast<uint2*>(codes + (row0 + row_of(r0 + j)) * D + cl * 8) =
+          make_uint2(pack4(u(n[0].x), u(n[0].y), u(n[1].x), u(n[1].y)),
+                     pack4(u(n[2].x), u(n[2].y), u(n[3].x), u(n[3].y)));
+    }
   }
 }
 

@@ -119,8 +119,10 @@ __device__ __forceinline__ unsigned pack4(unsigned a, unsigned b, unsigned c, un
 // byte of 2^23 + code, and one exact subtraction takes both offsets off (the
 // conversion instruction runs at an eighth of the rate).
 template <int I>
-__device__ __forceinline__ float code_f(unsigned biased) {   // biased = codes ^ 0x80808080
-  return __uint_as_float(__byte_perm(biased, 0x4b000000u, 0x7440 + I)) - 8388736.f;
+__device__ __forceinline__ float biased_f(unsigned biased) {   // biased = codes ^ 0x80808080
+  return __uint_as_float(__byte_perm(biased, 0x4b000000u, 0x7440 + I));
 }
+template <int I>
+__device__ __forceinline__ float code_f(unsigned biased) { return biased_f<I>(biased) - 8388736.f; }
 
 }  // namespace gdn2

@@ -282,7 +282,7 @@ int gdn2_state_read(int dtype, const void* codes, const float* scales, const int
  * slots lie outside the cache, or whose destination is another row's source or
  * destination, gets NaN outputs and stores nothing: its result would depend on
  * the order of blocks.  A state is taken as stored (the sanitiser acts as it is
- * written), a scale that is not finite as 0.  D is 64 or 128; codes and scales
+ * written), a NaN scale as 0.  D is 64 or 128; codes and scales
  * are 16-byte aligned. */
 int gdn2_decode_cached(int dtype, const void* q, const void* k, const void* v, const void* w,
                        const void* b, const void* g, void* codes, float* scales, const int* src,
