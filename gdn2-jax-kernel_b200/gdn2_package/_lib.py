@@ -156,6 +156,34 @@ def load():
     return lib
 
 
+def raw_stream(index):
+    """cudaStream_t of the current stream of CUDA device ``index``."""
+    import torch
+    get = getattr(torch._C, "_cuda_getCurrentRawStream", None)   # 2 us less than the object
+    return get(index) if get else torch.cuda.current_stream(index).cuda_stream
+
+
+class on_device:
+    """``torch.cuda.device`` for a device index, without its cost where that
+    device is the current one."""
+
+    __slots__ = ("index", "outer")
+
+    def __init__(self, index):
+        self.index = index
+
+    def __enter__(self):
+        import torch
+        self.outer = None
+        if torch.cuda.current_device() != self.index:
+            self.outer = torch.cuda.device(self.index)
+            self.outer.__enter__()
+
+    def __exit__(self, *exc):
+        if self.outer is not None:
+            self.outer.__exit__(*exc)
+
+
 def check(rc, what):
     if rc == OK:
         return

@@ -25,28 +25,43 @@ GROUP = 64         # values that share a scale
 _MAX_TENSORS = 8   # of one launch (GDN2_INT8_MAX_TENSORS)
 
 
-def _aligned(t):
-    """``t`` contiguous and on a 16-byte boundary."""
-    t = t.contiguous()
+def _operand(t, dev, dtype):
+    """``t`` on ``dev`` in ``dtype``, contiguous and on a 16-byte boundary."""
+    if t.dtype is not dtype or t.device != dev:
+        t = t.to(device=dev, dtype=dtype, non_blocking=True)
+    if not t.is_contiguous():
+        t = t.contiguous()
     return t.clone() if t.data_ptr() % 16 else t
 
 
 class Gdn2Checkpoint:
-    """Tensors in the int8 form: per tensor ``codes`` (its shape, int8) and
-    ``scales`` (its shape with the last axis divided by 64, float32)."""
+    """Tensors in the int8 form.  ``codes[i]`` (the tensor's shape, int8) and
+    ``scales[i]`` (its shape with the last axis divided by 64, float32) are views
+    of one buffer each per launch (``buffers``: (indexes, codes, scales))."""
 
-    __slots__ = ("codes", "scales", "dtypes", "on_host")
+    __slots__ = ("buffers", "shapes", "dtypes", "on_host")
 
-    def __init__(self, codes, scales, dtypes, on_host):
-        self.codes, self.scales, self.dtypes, self.on_host = codes, scales, dtypes, on_host
+    def __init__(self, buffers, shapes, dtypes, on_host):
+        self.buffers, self.shapes, self.dtypes, self.on_host = buffers, shapes, dtypes, on_host
+
+    def _views(self, which, last):
+        out = [None] * len(self.shapes)
+        for entry in self.buffers:
+            for j, i in enumerate(entry[0]):
+                s = self.shapes[i]
+                out[i] = entry[which][j].view((*s[:-1], s[-1] // last))
+        return out
+
+    codes = property(lambda self: self._views(1, 1))
+    scales = property(lambda self: self._views(2, GROUP))
 
     @property
     def nbytes(self):
-        return sum(c.numel() for c in self.codes) + 4 * sum(s.numel() for s in self.scales)
+        return sum(c.numel() + 4 * s.numel() for _, c, s in self.buffers)
 
 
-def _pointers(ts):
-    return (ctypes.c_void_p * len(ts))(*[t.data_ptr() for t in ts])
+def _pointers(ps):
+    return (ctypes.c_void_p * len(ps))(*ps)
 
 
 def _launches(dtypes, counts):
@@ -58,10 +73,16 @@ def _launches(dtypes, counts):
             for i in range(0, len(at), _MAX_TENSORS)]
 
 
+def _buffer_pointers(at, codes, scales, n):
+    c, s = codes.data_ptr(), scales.data_ptr()
+    return (_pointers([c + j * n for j in range(len(at))]),
+            _pointers([s + j * (n // GROUP * 4) for j in range(len(at))]))
+
+
 def gdn2_checkpoint_pack(*tensors):
     """The int8 form of ``tensors`` (floating point, last axis a multiple of
     64) as a ``Gdn2Checkpoint``.  Not differentiable."""
-    ts = [torch.as_tensor(t).detach() for t in tensors]
+    ts = [t if isinstance(t, torch.Tensor) else torch.as_tensor(t) for t in tensors]
     if not ts:
         raise _fwd.Gdn2ShapeError("no tensors to pack")
     for t in ts:
@@ -70,38 +91,38 @@ def gdn2_checkpoint_pack(*tensors):
         if t.dim() == 0 or t.shape[-1] % GROUP or t.numel() == 0:
             raise _fwd.Gdn2ShapeError(
                 f"the last axis must be a positive multiple of {GROUP}; got {tuple(t.shape)}")
-    on_host = ts[0].device.type != "cuda"
+    on_host = not ts[0].is_cuda
     dev = torch.device("cuda", torch.cuda.current_device()) if on_host else ts[0].device
-    x = [_aligned(t.to(device=dev, dtype=t.dtype if t.dtype == torch.bfloat16 else torch.float32,
-                       non_blocking=True)) for t in ts]
-    codes = [torch.empty(t.shape, dtype=torch.int8, device=dev) for t in x]
-    scales = [torch.empty((*t.shape[:-1], t.shape[-1] // GROUP), dtype=torch.float32, device=dev)
-              for t in x]
+    x = [_operand(t, dev, t.dtype if t.dtype is torch.bfloat16 else torch.float32) for t in ts]
     lib = _lib.load()
-    with torch.cuda.device(dev):
-        stream = _fwd._stream(dev)
+    buffers = []
+    with _lib.on_device(dev.index):
+        stream = _lib.raw_stream(dev.index)
         for (dt, n), at in _launches([t.dtype for t in x], [t.numel() for t in x]):
-            rc = lib.gdn2_int8_pack(_lib.BF16 if dt == torch.bfloat16 else _lib.F32, len(at),
-                                    _pointers([x[i] for i in at]),
-                                    _pointers([codes[i] for i in at]),
-                                    _pointers([scales[i] for i in at]), n, stream)
+            codes = torch.empty((len(at), n), dtype=torch.int8, device=dev)
+            scales = torch.empty((len(at), n // GROUP), dtype=torch.float32, device=dev)
+            rc = lib.gdn2_int8_pack(_lib.BF16 if dt is torch.bfloat16 else _lib.F32, len(at),
+                                    _pointers([x[i].data_ptr() for i in at]),
+                                    *_buffer_pointers(at, codes, scales, n), n, stream)
             _lib.check(rc, "gdn2_checkpoint_pack")
-    return Gdn2Checkpoint(codes, scales, [t.dtype for t in ts], on_host)
+            buffers.append((at, codes, scales))
+    return Gdn2Checkpoint(buffers, [t.shape for t in ts], [t.dtype for t in ts], on_host)
 
 
 def gdn2_checkpoint_unpack(kept):
     """The tensors that ``kept`` holds, each in the type it was packed from."""
-    dev = kept.codes[0].device
-    out = [torch.empty(c.shape, dtype=dt if dt == torch.bfloat16 else torch.float32, device=dev)
-           for c, dt in zip(kept.codes, kept.dtypes)]
+    dev = kept.buffers[0][1].device
+    out = [torch.empty(s, dtype=dt if dt is torch.bfloat16 else torch.float32, device=dev)
+           for s, dt in zip(kept.shapes, kept.dtypes)]
     lib = _lib.load()
-    with torch.cuda.device(dev):
-        stream = _fwd._stream(dev)
-        for (dt, n), at in _launches([t.dtype for t in out], [t.numel() for t in out]):
-            rc = lib.gdn2_int8_unpack(_lib.BF16 if dt == torch.bfloat16 else _lib.F32, len(at),
-                                      _pointers([out[i] for i in at]),
-                                      _pointers([kept.codes[i] for i in at]),
-                                      _pointers([kept.scales[i] for i in at]), n, stream)
+    with _lib.on_device(dev.index):
+        stream = _lib.raw_stream(dev.index)
+        for at, codes, scales in kept.buffers:
+            n = codes.shape[1]
+            rc = lib.gdn2_int8_unpack(
+                _lib.BF16 if out[at[0]].dtype is torch.bfloat16 else _lib.F32, len(at),
+                _pointers([out[i].data_ptr() for i in at]),
+                *_buffer_pointers(at, codes, scales, n), n, stream)
             _lib.check(rc, "gdn2_checkpoint_unpack")
-    out = [t.to(dt) for t, dt in zip(out, kept.dtypes)]
+    out = [t if t.dtype is dt else t.to(dt) for t, dt in zip(out, kept.dtypes)]
     return tuple(t.cpu() for t in out) if kept.on_host else tuple(out)

@@ -70,8 +70,9 @@ class _Gdn2CoreInt8(torch.autograd.Function):
     def forward(ctx, q, k, v, w, b, g, h0, scale):
         o, h_final = _fwd.gdn2_pallas_forward(q, k, v, w, b, g, scale, h0)
         kept = gdn2_checkpoint_pack(q, k, v, w, b)
-        ctx.scale, ctx.dtypes, ctx.on_host = scale, kept.dtypes, kept.on_host
-        ctx.save_for_backward(g, h0, *kept.codes, *kept.scales)
+        ctx.scale, ctx.shapes, ctx.dtypes, ctx.on_host = scale, kept.shapes, kept.dtypes, kept.on_host
+        ctx.at = [at for at, _, _ in kept.buffers]
+        ctx.save_for_backward(g, h0, *(t for _, *pair in kept.buffers for t in pair))
         return o, h_final
 
     @staticmethod
@@ -81,7 +82,8 @@ class _Gdn2CoreInt8(torch.autograd.Function):
         if do is None:
             do = torch.zeros(g.shape, dtype=torch.float32, device=g.device)
         q, k, v, w, b = gdn2_checkpoint_unpack(
-            Gdn2Checkpoint(kept[:5], kept[5:], ctx.dtypes, ctx.on_host))
+            Gdn2Checkpoint(list(zip(ctx.at, kept[::2], kept[1::2])), ctx.shapes, ctx.dtypes,
+                           ctx.on_host))
         grads = _bwd.gdn2_backward(q, k, v, w, b, g, ctx.scale, h0, do, dh_final)
         return *grads, None
 

@@ -21,7 +21,7 @@ import torch
 
 from . import _lib
 from . import gdn2_fwd as _fwd
-from .gdn2_checkpoint import GROUP, _aligned
+from .gdn2_checkpoint import GROUP, _operand
 
 INTERVAL = 64   # tokens between the states kept for the backward (GDN2_RECUR_INTERVAL)
 
@@ -33,55 +33,72 @@ class _Call:
                  "h0_dtype")
 
     def __init__(self, v, w, g, h0):
-        ts = (v, w, g)
-        if not all(isinstance(t, torch.Tensor) for t in ts):
-            ts = tuple(torch.as_tensor(t) for t in ts)
-        shape = tuple(ts[0].shape)
-        if len(shape) != 4 or any(tuple(t.shape) != shape for t in ts):
-            raise _fwd.Gdn2ShapeError(f"inputs must share one (B, T, H, D) shape; got {shape}")
+        if not (isinstance(v, torch.Tensor) and isinstance(w, torch.Tensor)
+                and isinstance(g, torch.Tensor)):
+            v, w, g = torch.as_tensor(v), torch.as_tensor(w), torch.as_tensor(g)
+        shape = v.shape
+        if len(shape) != 4 or w.shape != shape or g.shape != shape:
+            raise _fwd.Gdn2ShapeError(
+                f"inputs must share one (B, T, H, D) shape; got {tuple(shape)}")
         self.B, self.T, self.H, self.D = B, T, H, D = shape
         if D not in (64, 128, 256):
             raise _fwd.Gdn2ShapeError(f"head dim D={D} unsupported (64, 128 or 256)")
         if B * T * H == 0:
             raise _fwd.Gdn2ShapeError("empty problem")
-        self.dtypes = tuple(t.dtype for t in ts)
-        if any(not dt.is_floating_point for dt in self.dtypes):
+        vt, wt, gt = self.dtypes = (v.dtype, w.dtype, g.dtype)
+        if not (vt.is_floating_point and wt.is_floating_point and gt.is_floating_point):
             raise _fwd.Gdn2ShapeError("inputs must be floating point")
-        if _fwd.GATES not in ("activated", "raw"):
-            raise _fwd.Gdn2ShapeError(f"GATES={_fwd.GATES!r}: 'activated' or 'raw'")
-        self.on_host = ts[0].device.type != "cuda"
+        gates = _fwd.GATES
+        if gates not in ("activated", "raw"):
+            raise _fwd.Gdn2ShapeError(f"GATES={gates!r}: 'activated' or 'raw'")
+        self.on_host = not v.is_cuda
         self.dev = dev = (torch.device("cuda", torch.cuda.current_device()) if self.on_host
-                          else ts[0].device)
-        bf16 = all(dt == torch.bfloat16 for dt in self.dtypes)
+                          else v.device)
+        bf16 = vt is wt is gt is torch.bfloat16
         cdt = torch.bfloat16 if bf16 else torch.float32
-        self.code = (_lib.BF16 if bf16 else _lib.F32) | (_lib.GATES_RAW if _fwd.GATES == "raw" else 0)
-        self.v, self.w, self.g = (_aligned(t.to(device=dev, dtype=cdt, non_blocking=True))
-                                  for t in ts)
+        self.code = (_lib.BF16 if bf16 else _lib.F32) | (_lib.GATES_RAW if gates == "raw" else 0)
+        self.v, self.w, self.g = _operand(v, dev, cdt), _operand(w, dev, cdt), _operand(g, dev, cdt)
         self.h0 = self.h0_dtype = None
         if h0 is not None:
-            h0 = torch.as_tensor(h0)
-            if tuple(h0.shape) != (B, H, D):
+            if not isinstance(h0, torch.Tensor):
+                h0 = torch.as_tensor(h0)
+            if h0.shape != (B, H, D):
                 raise _fwd.Gdn2ShapeError(f"h0 must be {(B, H, D)}; got {tuple(h0.shape)}")
             self.h0_dtype = h0.dtype
-            self.h0 = _aligned(h0.to(device=dev, dtype=torch.float32, non_blocking=True))
+            self.h0 = _operand(h0, dev, torch.float32)
 
 
 class Gdn2RecurrenceResiduals:
-    """What the backward of one forward needs: g, v and w or their int8 form,
-    and the state before every 64th token."""
+    """What the backward of one forward needs: g, v and w or their int8 form
+    (codes (2, B, T, H, D) and scales (2, B, T, H, D / 64)), and ``kept``, the
+    state before every 64th token."""
 
-    __slots__ = ("B", "T", "H", "D", "dev", "on_host", "code", "dtypes", "h0_dtype", "g", "v", "w",
-                 "int8", "kept")
+    __slots__ = ("shape", "dev", "on_host", "code", "dtypes", "h0_dtype", "g", "v", "w", "int8",
+                 "kept")
 
     def __init__(self, c, int8, kept):
-        for n in ("B", "T", "H", "D", "dev", "on_host", "code", "dtypes", "h0_dtype", "g"):
-            setattr(self, n, getattr(c, n))
-        self.v, self.w = (None, None) if int8 else (c.v, c.w)
-        self.int8, self.kept = int8, kept   # int8: (v codes, v scales, w codes, w scales)
+        self.shape, self.dev, self.on_host = (c.B, c.T, c.H, c.D), c.dev, c.on_host
+        self.code, self.dtypes, self.h0_dtype = c.code, c.dtypes, c.h0_dtype
+        self.g, self.v, self.w = c.g, None if int8 else c.v, None if int8 else c.w
+        self.int8, self.kept = int8, kept
+
+    def without_tensors(self):
+        """The sizes and types alone, for a copy that ``with_tensors`` completes."""
+        return (self.shape, self.dev, self.on_host, self.code, self.dtypes, self.h0_dtype,
+                self.int8 is not None)
+
+    @classmethod
+    def with_tensors(cls, rest, g, kept, *pair):
+        self = cls.__new__(cls)
+        (self.shape, self.dev, self.on_host, self.code, self.dtypes, self.h0_dtype, int8) = rest
+        self.g, self.kept = g, kept
+        self.int8 = pair if int8 else None
+        self.v, self.w = (None, None) if int8 else pair
+        return self
 
     @property
     def nbytes(self):
-        ts = [self.g, self.kept, *(self.int8 if self.int8 else (self.v, self.w))]
+        ts = [self.g, self.kept, *(self.int8 or (self.v, self.w))]
         return sum(t.numel() * t.element_size() for t in ts)
 
 
@@ -89,35 +106,42 @@ def _ptr(t):
     return t.data_ptr() if t is not None else None
 
 
-def _workspace(lib, c):
+def _int8_pointers(packed):
+    """Codes and scales of v, then of w."""
+    if packed is None:
+        return None, None, None, None
+    codes, scales = packed
+    c, s, n = codes.data_ptr(), scales.data_ptr(), codes.numel() // 2
+    return c, s, c + n, s + n // GROUP * 4
+
+
+def _workspace(lib, shape, dev):
     """Scratch of one call; none where the sequence is one tile."""
-    if c.T <= INTERVAL:
+    if shape[1] <= INTERVAL:
         return None, 0
-    n = lib.gdn2_recur_workspace_bytes(c.B, c.T, c.H, c.D)
+    n = lib.gdn2_recur_workspace_bytes(*shape)
     if n == 0:
         raise _fwd.Gdn2ShapeError("invalid sizes for the workspace")
-    return torch.empty(n, dtype=torch.uint8, device=c.dev), n
+    return torch.empty(n, dtype=torch.uint8, device=dev), n
 
 
 def _forward(c, keep, int8):
     lib = _lib.load()
     B, T, H, D, dev = c.B, c.T, c.H, c.D, c.dev
-    o = torch.empty((B, T, H, D), dtype=torch.float32, device=dev)
+    o = torch.empty_like(c.v, dtype=torch.float32)
     hf = torch.empty((B, H, D), dtype=torch.float32, device=dev)
     kept = packed = None
     if keep:
         kept = torch.empty((B, -(-T // INTERVAL), H, D), dtype=torch.float32, device=dev)
         if int8:
-            packed = tuple(torch.empty(s, dtype=dt, device=dev) for _ in range(2)
-                           for s, dt in (((B, T, H, D), torch.int8),
-                                         ((B, T, H, D // GROUP), torch.float32)))
-    ws, n = _workspace(lib, c)
-    with torch.cuda.device(dev):
-        stream = _fwd._stream(dev)
+            packed = (torch.empty((2, B, T, H, D), dtype=torch.int8, device=dev),
+                      torch.empty((2, B, T, H, D // GROUP), dtype=torch.float32, device=dev))
+    with _lib.on_device(dev.index):
+        ws, n = _workspace(lib, (B, T, H, D), dev)
+        stream = _lib.raw_stream(dev.index)
         rc = lib.gdn2_recur_fwd(c.code, c.v.data_ptr(), c.w.data_ptr(), c.g.data_ptr(), _ptr(c.h0),
-                                o.data_ptr(), hf.data_ptr(), _ptr(kept),
-                                *(map(_ptr, packed) if packed else (None,) * 4), _ptr(ws), n,
-                                B, T, H, D, stream)
+                                o.data_ptr(), hf.data_ptr(), _ptr(kept), *_int8_pointers(packed),
+                                _ptr(ws), n, B, T, H, D, stream)
         _lib.check(rc, "gdn2_linear_recurrence")
         if ws is not None:
             _lib.check_status(ws, stream, "gdn2_linear_recurrence", synced=c.on_host)
@@ -151,35 +175,34 @@ def gdn2_linear_recurrence_backward(residuals, dout, dh_final=None):
     type (dh0 float32 where h0 was not given).  With int8 residuals these are the
     gradients at the restored v and w, from the forward's states every 64
     tokens."""
-    r = residuals
-    shape = (r.B, r.T, r.H, r.D)
-    f32 = dict(device=r.dev, dtype=torch.float32, non_blocking=True)
-    dout = torch.as_tensor(dout)
-    if tuple(dout.shape) != shape:
-        raise _fwd.Gdn2ShapeError(f"dout must be {shape}; got {tuple(dout.shape)}")
-    do = _aligned(dout.to(**f32))
-    dh = None
+    r, dev = residuals, residuals.dev
+    B, T, H, D = r.shape
+    if not isinstance(dout, torch.Tensor):
+        dout = torch.as_tensor(dout)
+    if dout.shape != r.shape:
+        raise _fwd.Gdn2ShapeError(f"dout must be {r.shape}; got {tuple(dout.shape)}")
+    do, dh = _operand(dout, dev, torch.float32), None
     if dh_final is not None:
-        dh_final = torch.as_tensor(dh_final)
-        if tuple(dh_final.shape) != (r.B, r.H, r.D):
-            raise _fwd.Gdn2ShapeError(f"dh_final must be {(r.B, r.H, r.D)}")
-        dh = _aligned(dh_final.to(**f32))
+        if not isinstance(dh_final, torch.Tensor):
+            dh_final = torch.as_tensor(dh_final)
+        if dh_final.shape != (B, H, D):
+            raise _fwd.Gdn2ShapeError(f"dh_final must be {(B, H, D)}")
+        dh = _operand(dh_final, dev, torch.float32)
     lib = _lib.load()
-    dv, dw, dg = (torch.empty(shape, dtype=r.g.dtype, device=r.dev) for _ in range(3))
-    dh0 = torch.empty((r.B, r.H, r.D), dtype=torch.float32, device=r.dev)
-    ws, n = _workspace(lib, r)
-    with torch.cuda.device(r.dev):
-        stream = _fwd._stream(r.dev)
+    dv, dw, dg = torch.empty_like(r.g), torch.empty_like(r.g), torch.empty_like(r.g)
+    dh0 = torch.empty((B, H, D), dtype=torch.float32, device=dev)
+    with _lib.on_device(dev.index):
+        ws, n = _workspace(lib, r.shape, dev)
+        stream = _lib.raw_stream(dev.index)
         rc = lib.gdn2_recur_bwd(r.code, _ptr(r.v), _ptr(r.w), r.g.data_ptr(),
-                                *(map(_ptr, r.int8) if r.int8 else (None,) * 4),
-                                r.kept.data_ptr(), do.data_ptr(), _ptr(dh), dv.data_ptr(),
-                                dw.data_ptr(), dg.data_ptr(), dh0.data_ptr(), _ptr(ws), n,
-                                r.B, r.T, r.H, r.D, stream)
+                                *_int8_pointers(r.int8), r.kept.data_ptr(), do.data_ptr(),
+                                _ptr(dh), dv.data_ptr(), dw.data_ptr(), dg.data_ptr(),
+                                dh0.data_ptr(), _ptr(ws), n, B, T, H, D, stream)
         _lib.check(rc, "gdn2_linear_recurrence_backward")
         if ws is not None:
             _lib.check_status(ws, stream, "gdn2_linear_recurrence_backward", synced=r.on_host)
-    out = [t.to(dt) for t, dt in zip((dv, dw, dg), r.dtypes)]
-    out.append(dh0 if r.h0_dtype is None else dh0.to(r.h0_dtype))
+    out = [t if t.dtype is dt else t.to(dt)
+           for t, dt in zip((dv, dw, dg, dh0), (*r.dtypes, r.h0_dtype or torch.float32))]
     return tuple(t.cpu() for t in out) if r.on_host else tuple(out)
 
 
@@ -190,9 +213,8 @@ class _Recurrence(torch.autograd.Function):
         c = _Call(v, w, g, h0)
         o, hf, res = _forward(c, True, int8)
         # through save_for_backward, which notices inputs that change in place
-        ctx.save_for_backward(res.g, res.kept, *(res.int8 if int8 else (res.v, res.w)))
-        res.g = res.kept = res.int8 = res.v = res.w = None
-        ctx.res, ctx.int8 = res, int8
+        ctx.save_for_backward(res.g, res.kept, *(res.int8 or (res.v, res.w)))
+        ctx.rest = res.without_tensors()
         return (o.cpu(), hf.cpu()) if c.on_host else (o, hf)
 
     @staticmethod
@@ -200,15 +222,9 @@ class _Recurrence(torch.autograd.Function):
     def backward(ctx, do, dh):
         if do is None and dh is None:
             return (None,) * 5
-        saved = ctx.saved_tensors
-        c, r = ctx.res, Gdn2RecurrenceResiduals.__new__(Gdn2RecurrenceResiduals)
-        for n in ("B", "T", "H", "D", "dev", "on_host", "code", "dtypes", "h0_dtype"):
-            setattr(r, n, getattr(c, n))
-        r.g, r.kept = saved[:2]
-        r.int8 = tuple(saved[2:]) if ctx.int8 else None
-        r.v, r.w = (None, None) if ctx.int8 else saved[2:]
+        r = Gdn2RecurrenceResiduals.with_tensors(ctx.rest, *ctx.saved_tensors)
         if do is None:
-            do = torch.zeros((r.B, r.T, r.H, r.D), dtype=torch.float32, device=r.dev)
+            do = torch.zeros(r.shape, dtype=torch.float32, device=r.dev)
         dv, dw, dg, dh0 = gdn2_linear_recurrence_backward(r, do, dh)
         return dv, dw, dg, None if r.h0_dtype is None else dh0, None
 

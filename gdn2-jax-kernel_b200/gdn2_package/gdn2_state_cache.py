@@ -23,7 +23,7 @@ import torch
 
 from . import _lib
 from . import gdn2_fwd as _fwd
-from .gdn2_checkpoint import GROUP, _aligned
+from .gdn2_checkpoint import GROUP, _operand
 
 
 class Gdn2StateCache:
@@ -66,7 +66,7 @@ class Gdn2StateCache:
 
 
 def _on_gpu(cache):
-    if cache.codes.device.type != "cuda":
+    if not cache.codes.is_cuda:
         raise _fwd.Gdn2ShapeError("the cache must be on a CUDA device")
     return cache.codes.device
 
@@ -88,7 +88,9 @@ def _slots(slots, B, S, dev, what, distinct):
         if B > S:
             raise _fwd.Gdn2ShapeError(f"{B} rows for {S} slots: give {what}")
         return None, None
-    on_gpu = isinstance(slots, torch.Tensor) and slots.device.type == "cuda"
+    on_gpu = isinstance(slots, torch.Tensor) and slots.is_cuda
+    if on_gpu and slots.dtype is torch.int32 and slots.shape == (B,) and slots.device == dev:
+        return slots.contiguous(), None
     t = slots if isinstance(slots, torch.Tensor) else torch.as_tensor(slots)
     if t.dtype not in (torch.int32, torch.int64) or tuple(t.shape) != (B,):
         raise _fwd.Gdn2ShapeError(f"{what} must be {B} int32 or int64 values; "
@@ -109,17 +111,18 @@ def gdn2_state_write(cache, h, slots=None):
     by default), through the CLIP sanitiser.  Of several rows that name one slot
     the last is kept (slots on the host must be distinct)."""
     dev = _on_gpu(cache)
-    h = torch.as_tensor(h)
-    if h.dim() != 4 or tuple(h.shape[1:]) != tuple(cache.codes.shape[1:]) or h.shape[0] == 0:
+    if not isinstance(h, torch.Tensor):
+        h = torch.as_tensor(h)
+    if h.dim() != 4 or h.shape[1:] != cache.codes.shape[1:] or h.shape[0] == 0:
         raise _fwd.Gdn2ShapeError(
             f"h must be (B, {cache.H}, {cache.D}, {cache.D}); got {tuple(h.shape)}")
     B, S = h.shape[0], cache.slots
     at, _ = _slots(slots, B, S, dev, "slots", True)
-    hs = _aligned(h.detach().to(device=dev, dtype=torch.float32, non_blocking=True))
-    with torch.cuda.device(dev):
+    hs = _operand(h, dev, torch.float32)
+    with _lib.on_device(dev.index):
         rc = _lib.load().gdn2_state_write(hs.data_ptr(), _ptr(at), cache.codes.data_ptr(),
                                           cache.scales.data_ptr(), B, S, cache.H, cache.D,
-                                          float(_fwd.CLIP), _fwd._stream(dev))
+                                          float(_fwd.CLIP), _lib.raw_stream(dev.index))
     _lib.check(rc, "gdn2_state_write")
 
 
@@ -135,10 +138,10 @@ def gdn2_state_read(cache, slots=None, dtype=torch.float32):
         raise _fwd.Gdn2ShapeError("empty problem")
     at, _ = _slots(slots, B, S, dev, "slots", False)
     h = torch.empty((B, H, D, D), dtype=dtype, device=dev)
-    with torch.cuda.device(dev):
+    with _lib.on_device(dev.index):
         rc = _lib.load().gdn2_state_read(_lib.F32 if dtype == torch.float32 else _lib.BF16,
                                          cache.codes.data_ptr(), cache.scales.data_ptr(), _ptr(at),
-                                         h.data_ptr(), B, S, H, D, _fwd._stream(dev))
+                                         h.data_ptr(), B, S, H, D, _lib.raw_stream(dev.index))
     _lib.check(rc, "gdn2_state_read")
     return h
 
@@ -153,10 +156,12 @@ def gdn2_decode_cached(q, k, v, w, b, g, scale, cache, slots=None, out_slots=Non
     destination: the host refuses such slots where it has them, the kernel gives
     NaN for the row and stores nothing."""
     dev = _on_gpu(cache)
-    ts = tuple(torch.as_tensor(t) for t in (q, k, v, w, b, g))
-    shape = tuple(ts[0].shape)
-    if len(shape) != 4 or any(tuple(t.shape) != shape for t in ts):
-        raise _fwd.Gdn2ShapeError(f"inputs must share one (B, T, H, D) shape; got {shape}")
+    ts = (q, k, v, w, b, g)
+    if not all(isinstance(t, torch.Tensor) for t in ts):
+        ts = tuple(torch.as_tensor(t) for t in ts)
+    shape = ts[0].shape
+    if len(shape) != 4 or any(t.shape != shape for t in ts):
+        raise _fwd.Gdn2ShapeError(f"inputs must share one (B, T, H, D) shape; got {tuple(shape)}")
     B, T, H, D = shape
     if D not in (64, 128):
         raise _fwd.Gdn2ShapeError(f"head dim D={D} unsupported (64 or 128)")
@@ -164,10 +169,10 @@ def gdn2_decode_cached(q, k, v, w, b, g, scale, cache, slots=None, out_slots=Non
         raise _fwd.Gdn2ShapeError("empty problem")
     if any(not t.dtype.is_floating_point for t in ts):
         raise _fwd.Gdn2ShapeError("inputs must be floating point")
-    if (H, D) != (cache.H, cache.D):
+    if cache.codes.shape[1:3] != (H, D):
         raise _fwd.Gdn2ShapeError(f"the cache holds states of H={cache.H}, D={cache.D}; "
                                   f"got H={H}, D={D}")
-    S = cache.slots
+    S = cache.codes.shape[0]
     if slots is None and out_slots is not None:
         raise _fwd.Gdn2ShapeError("out_slots need slots")
     src, src_host = _slots(slots, B, S, dev, "slots", out_slots is None)
@@ -180,17 +185,17 @@ def gdn2_decode_cached(q, k, v, w, b, g, scale, cache, slots=None, out_slots=Non
                 readers.setdefault(s, []).append(i)
             if any(d >= 0 and any(j != i for j in readers.get(d, ())) for i, d in enumerate(dst_host)):
                 raise _fwd.Gdn2ShapeError("a slot of out_slots is another row's slot")
-    on_host = ts[0].device.type != "cuda"
-    cdt = torch.bfloat16 if all(t.dtype == torch.bfloat16 for t in ts) else torch.float32
-    x = [t.to(device=dev, dtype=cdt, non_blocking=True).contiguous() for t in ts]
-    o = torch.empty((B, T, H, D), dtype=torch.float32, device=dev)
-    code = _lib.F32 if cdt == torch.float32 else _lib.BF16
+    bf16 = all(t.dtype is torch.bfloat16 for t in ts)
+    cdt = torch.bfloat16 if bf16 else torch.float32
+    x = [_operand(t, dev, cdt) for t in ts]
+    o = torch.empty(shape, dtype=torch.float32, device=dev)
+    code = _lib.BF16 if bf16 else _lib.F32
     if _fwd.GATES == "raw":
         code |= _lib.GATES_RAW
-    with torch.cuda.device(dev):
+    with _lib.on_device(dev.index):
         rc = _lib.load().gdn2_decode_cached(
             code, *[t.data_ptr() for t in x], cache.codes.data_ptr(), cache.scales.data_ptr(),
             _ptr(src), _ptr(dst), o.data_ptr(), B, T, H, D, S, float(scale), float(_fwd.CLIP),
-            _fwd._stream(dev))
+            _lib.raw_stream(dev.index))
     _lib.check(rc, "gdn2_decode_cached")
-    return o.cpu() if on_host else o
+    return o if ts[0].is_cuda else o.cpu()
