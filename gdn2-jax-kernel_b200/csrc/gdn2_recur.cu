@@ -22,10 +22,15 @@
 // there.  The last tile of a group publishes the state that enters the next.
 // So a sequence of n tiles is n / 16 dependent steps, every state is formed by
 // the same operations whatever ran first (results do not depend on timing),
-// and a tile reads at most 16 published maps of 512 bytes.  Tiles are taken in
-// the order of time by a counter, so what a tile waits for has always started.
-// A published word is 64 bits, (a, b) of one channel, with the sign bit of a
-// (never negative) set: zeroed memory is "not yet", and no fence is needed.
+// and a tile reads at most 16 published maps of 512 bytes.  A published word is
+// 64 bits, (a, b) of one channel, with the sign bit of a (never negative) set:
+// zeroed memory is "not yet", and no fence is needed.
+//
+// What a tile waits for is resolved by others while its CTA works: a CTA folds
+// and publishes the next tile before it finishes the present one, and the bytes
+// of the tile after that are on their way to shared memory.  (With the join in
+// the way of the loads the same kernels reached 73% and 80% of the copy rate,
+// without any join 95% and 100%.)
 //
 // The forward keeps the state that enters each tile (1/64 of o).  The backward
 // rebuilds the states inside a tile from it, so it does not read o; with int8
@@ -58,7 +63,33 @@ template <> struct Raw<__nv_bfloat16> { using type = unsigned; };
 template <> struct Raw<int8_t> { using type = unsigned short; };
 template <typename T>
 __device__ __forceinline__ typename Raw<T>::type ldraw(const T* p) {
-  return __ldcs(reinterpret_cast<const typename Raw<T>::type*>(p));
+  return *reinterpret_cast<const typename Raw<T>::type*>(p);
+}
+
+// Asynchronous copies to shared memory of 8 rows of 64 channels by one warp;
+// rows behind the end are left as they are.
+template <typename T>
+__device__ __forceinline__ void fetch(T* to, const T* from, size_t stride, int rows, int lane) {
+  constexpr int kPieces = kGroup * sizeof(T) / 16, kAt = 32 / kPieces;   // of a row; rows at once
+#pragma unroll
+  for (int r0 = 0; r0 < kRows; r0 += kAt) {
+    const int r = r0 + lane / kPieces, c = lane % kPieces * (16 / sizeof(T));
+    if (r < rows)
+      asm volatile("cp.async.cg.shared.global [%0], [%1], 16;"
+                   ::"r"((unsigned)__cvta_generic_to_shared(to + r * kGroup + c)),
+                     "l"(from + r * stride + c) : "memory");
+  }
+}
+__device__ __forceinline__ void fetch4(float* to, const float* from) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4;"
+               ::"r"((unsigned)__cvta_generic_to_shared(to)), "l"(from) : "memory");
+}
+__device__ __forceinline__ void fetch_end() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+// All fetches but the latest `N` have landed, for the whole warp.
+template <int N>
+__device__ __forceinline__ void fetched() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+  __syncwarp();
 }
 __device__ __forceinline__ float2 value2(float2 v) { return v; }
 __device__ __forceinline__ float2 value2(unsigned u) {
@@ -152,72 +183,116 @@ struct Args {
   int T, HD, tiles, chains;
 };
 
-// The tile of this CTA: (chain, index k in the order of the scan).
+// Tiles are taken in the order of time: ticket t is tile t / chains of chain
+// t % chains, in the order of the scan.  A CTA holds the tile it works on and the
+// next one, whose bytes are on their way meanwhile; what a tile waits for has a
+// lower ticket, and the lowest unfinished ticket is always being worked on.
+// Sequences of one tile wait for nothing and are dealt out by index.
 struct Place { int chain, k; };
-__device__ __forceinline__ Place take_tile(const Args& p) {
-  __shared__ int ticket;
-  unsigned t = blockIdx.x;
-  if (p.tiles > 1) {
-    if (threadIdx.x == 0) ticket = atomicAdd(p.s.status + 8, 1);
+struct Tickets {
+  int total;
+  bool drawn, more;   // from the counter; more than one a CTA
+  __device__ __forceinline__ Tickets(const Args& p)
+      : total(p.tiles * p.chains), drawn(p.tiles > 1), more(total > (int)gridDim.x) {}
+  __device__ __forceinline__ int draw(const Args& p) const { return atomicAdd(p.s.status + 8, 1); }
+  __device__ __forceinline__ int first(const Args& p, int* shared) const {
+    if (!drawn) return blockIdx.x;
+    if (threadIdx.x == 0) *shared = draw(p);
     __syncthreads();
-    t = (unsigned)ticket;
+    return *shared;
   }
-  return {(int)(t % p.chains), (int)(t / p.chains)};
-}
-
-// The state that enters tile k of a chain, from the maps of its warps in the
-// order of the scan (map, complete: the caller has synchronised) and `first`,
-// the state that enters the sequence.
-struct Joint {
-  float4 mates[kGroupTiles][32];
-  float2 enter[32];
+  // Drawn once the first tile's bytes are there, when other CTAs have theirs:
+  // one that drew two at once would leave another without any.
+  __device__ __forceinline__ int second(const Args& p, int* shared, int now) const {
+    if (!more) return total;
+    if (!drawn) return now + gridDim.x;
+    if (threadIdx.x == 0) *shared = draw(p);
+    __syncthreads();
+    return *shared;
+  }
+  __device__ __forceinline__ bool is(int t) const { return t < total; }
+  __device__ __forceinline__ Place place(const Args& p, int t) const {
+    return {(int)((unsigned)t % p.chains), (int)((unsigned)t / p.chains)};
+  }
 };
-__device__ __forceinline__ float2 enter_tile(const Args& p, const Place at,
-                                             const float4 (*map)[32], Joint& joint,
-                                             const float* first) {
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int mate = at.k % kGroupTiles, group = at.k / kGroupTiles;
-  const bool last = at.k + 1 == p.tiles, hands_on = mate == kGroupTiles - 1 && !last;
-  if (warp == 0 && !last && !hands_on) {
-    Map m = unflat(map[0][lane]);
+
+// How a tile of a chain gets the state that enters it (map: the maps of its warps
+// in the order of the scan).
+struct Joint {
+  float4 pairs[kWarps][32];   // the mates 2 w and 2 w + 1 before it in its group
+  float2 enter[32];           // the state that enters the group
+  int ticket[2];
+};
+__device__ __forceinline__ ulonglong2* map_of(const Args& p, Place at, int k, int lane) {
+  return p.s.maps + ((size_t)k * p.chains + at.chain) * 32 + lane;
+}
+__device__ __forceinline__ ulonglong2* enter_of(const Args& p, Place at, int group, int lane) {
+  return p.s.enter + ((size_t)group * p.chains + at.chain) * 32 + lane;
+}
+// One warp publishes a tile's map, where another tile will look at it.
+__device__ __forceinline__ void publish_map(const Args& p, Place at, const float4 (*map)[32], int lane) {
+  if (at.k + 1 == p.tiles || at.k % kGroupTiles == kGroupTiles - 1) return;
+  Map m = unflat(map[0][lane]);
 #pragma unroll
-    for (int j = 1; j < kWarps; ++j) m = after(unflat(map[j][lane]), m);
-    publish(p.s.maps + ((size_t)at.k * p.chains + at.chain) * 32 + lane, m);
-  }
-  const ulonglong2* mine = p.s.maps + ((size_t)(at.k - mate) * p.chains + at.chain) * 32 + lane;
-  const size_t next = (size_t)p.chains * 32;
-  if (warp < mate) {   // two waits at once: the second has mostly come when the first has
-    const bool two = warp + kWarps < mate;
-    const ulonglong2 second = two ? peek(mine + (warp + kWarps) * next) : ulonglong2{};
-    joint.mates[warp][lane] = flat(await(mine + warp * next, p.s.status));
-    if (two)
-      joint.mates[warp + kWarps][lane] =
-          flat(__all_sync(0xffffffffu, there(second)) ? unword(second)
-                                                      : await(mine + (warp + kWarps) * next, p.s.status));
-  }
-  if (mate) __syncthreads();
-  if (warp == 0) {
+  for (int j = 1; j < kWarps; ++j) m = after(unflat(map[j][lane]), m);
+  publish(map_of(p, at, at.k, lane), m);
+}
+// What a warp needs of others, looked at long before it is needed.
+struct Early { ulonglong2 even, odd, enter; };
+__device__ __forceinline__ Early look(const Args& p, Place at, int warp, int lane) {
+  const int mate = at.k % kGroupTiles, group = at.k / kGroupTiles;
+  Early e{};
+  if (2 * warp < mate) e.even = peek(map_of(p, at, at.k - mate + 2 * warp, lane));
+  if (2 * warp + 1 < mate) e.odd = peek(map_of(p, at, at.k - mate + 2 * warp + 1, lane));
+  if (warp == 0 && group) e.enter = peek(enter_of(p, at, group, lane));
+  return e;
+}
+__device__ __forceinline__ Map have(ulonglong2 early, const ulonglong2* p, int* status) {
+  return __all_sync(0xffffffffu, there(early)) ? unword(early) : await(p, status);
+}
+// All warps, between two synchronisations of the CTA; fills `joint`.
+__device__ __forceinline__ void join(const Args& p, Place at, const float4 (*map)[32], Joint& joint,
+                                     const float* first, const Early& e, int warp, int lane) {
+  const int mate = at.k % kGroupTiles, group = at.k / kGroupTiles, k0 = at.k - mate + 2 * warp;
+  const bool hands_on = mate == kGroupTiles - 1 && at.k + 1 < p.tiles;
+  Map m = identity();
+  if (2 * warp < mate) m = have(e.even, map_of(p, at, k0, lane), p.s.status);
+  if (2 * warp + 1 < mate) m = after(have(e.odd, map_of(p, at, k0 + 1, lane), p.s.status), m);
+  joint.pairs[warp][lane] = flat(m);
+  if (hands_on) {
     // the step from group to group is the dependent one: everything else of it
     // is joined before the wait
-    Map m = identity();
-    if (hands_on) {
-      for (int i = 0; i < mate; ++i) m = after(unflat(joint.mates[i][lane]), m);
+    __syncthreads();
+    if (warp == 0) {
+#pragma unroll
+      for (int i = 1; i < kWarps; ++i) m = after(unflat(joint.pairs[i][lane]), m);
 #pragma unroll
       for (int j = 0; j < kWarps; ++j) m = after(unflat(map[j][lane]), m);
     }
+  }
+  if (warp == 0) {
     float2 h = both(0.f);
     if (group)
-      h = await(p.s.enter + ((size_t)group * p.chains + at.chain) * 32 + lane, p.s.status).b;
+      h = have(e.enter, enter_of(p, at, group, lane), p.s.status).b;
     else if (first)
       h = *reinterpret_cast<const float2*>(first + (size_t)at.chain * kGroup + 2 * lane);
-    if (hands_on)
-      publish(p.s.enter + ((size_t)(group + 1) * p.chains + at.chain) * 32 + lane,
-              {both(0.f), apply(m, h)});
+    if (hands_on) publish(enter_of(p, at, group + 1, lane), {both(0.f), apply(m, h)});
     joint.enter[lane] = h;
   }
-  __syncthreads();
+}
+__device__ __forceinline__ float2 entering(const Joint& joint, int lane) {
   float2 h = joint.enter[lane];
-  for (int i = 0; i < mate; ++i) h = apply(unflat(joint.mates[i][lane]), h);
+#pragma unroll
+  for (int i = 0; i < kWarps; ++i) h = apply(unflat(joint.pairs[i][lane]), h);
+  return h;
+}
+// Through the maps of a tile's warps before `count`.
+__device__ __forceinline__ float2 walk(const float4 (*map)[32], int count, int lane, float2 h) {
+#pragma unroll
+  for (int j = 0; j < kWarps - 1; ++j) {
+    const float2 x = apply(unflat(map[j][lane]), h);
+    h = j < count ? x : h;
+  }
   return h;
 }
 
@@ -243,164 +318,358 @@ __device__ __forceinline__ float put_int8(const float2 (&v)[kRows], const float2
   return group_scale(mine);
 }
 
+// Where a tile lies for a warp: rows of it (8 and more: all eight), first element.
+struct Rows { int t0, rows; size_t i; };
+__device__ __forceinline__ Rows rows_of(const Args& p, Place at, int tile, int warp) {
+  const int groups = p.HD / kGroup, t0 = tile * kTile + warp * kRows;
+  return {t0, p.T - t0,
+          ((size_t)(at.chain / groups) * p.T + t0) * p.HD + at.chain % groups * kGroup};
+}
+
+// Shared memory of a warp: its 8 rows of the tile that comes next.
+template <typename T> struct FwdStage { T g[kRows][kGroup], v[kRows][kGroup], w[kRows][kGroup]; };
+
 template <typename T, bool SAVE8, bool RAW>
-__global__ void __launch_bounds__(256) k_recur_fwd(const Args p) {
-  __shared__ float4 map[kWarps][32];   // (a, b) of two channels
+__global__ void __launch_bounds__(256, 2) k_recur_fwd(const Args p) {
+  extern __shared__ __align__(16) unsigned char raw_stage[];
+  __shared__ float4 maps[3][kWarps][32];   // of the present tile, the next and the one before
   __shared__ Joint joint;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const Place at = take_tile(p);
-  const int groups = p.HD / kGroup, bb = at.chain / groups, cg = at.chain % groups;
-  const int ch = cg * kGroup + 2 * lane, t0 = at.k * kTile + warp * kRows;
-  const int rows = min(kRows, p.T - t0);   // of this warp; below 1: none
-  const size_t i0 = ((size_t)bb * p.T + t0) * p.HD + ch;
-  float2 a[kRows], x[kRows];
-  if (rows > 0) {
-    // every load before any arithmetic; rows behind the end read the last one
+  FwdStage<T>& st = reinterpret_cast<FwdStage<T>*>(raw_stage)[warp];
+  const int groups = p.HD / kGroup;
+  const Tickets tickets(p);
+  auto prefetch = [&](int t) {
+    if (tickets.is(t)) {
+      const Place at = tickets.place(p, t);
+      const Rows z = rows_of(p, at, at.k, warp);
+      fetch(&st.g[0][0], static_cast<const T*>(p.g) + z.i, p.HD, z.rows, lane);
+      fetch(&st.v[0][0], static_cast<const T*>(p.v) + z.i, p.HD, z.rows, lane);
+      fetch(&st.w[0][0], static_cast<const T*>(p.w) + z.i, p.HD, z.rows, lane);
+    }
+    fetch_end();
+  };
+  // the rows of tile t as maps (a, x), and the map of the warp
+  auto fold = [&](int t, float2 (&a)[kRows], float2 (&x)[kRows], float4 (*map)[32]) {
+    const Place at = tickets.place(p, t);
+    const Rows z = rows_of(p, at, at.k, warp);
     typename Raw<T>::type rg[kRows], rv[kRows], rw[kRows];
+    fetched<0>();
 #pragma unroll
     for (int r = 0; r < kRows; ++r) {
-      const size_t i = i0 + (size_t)min(r, rows - 1) * p.HD;
-      rg[r] = ldraw(static_cast<const T*>(p.g) + i);
-      rv[r] = ldraw(static_cast<const T*>(p.v) + i);
-      rw[r] = ldraw(static_cast<const T*>(p.w) + i);
+      rg[r] = ldraw(&st.g[r][2 * lane]);
+      rv[r] = ldraw(&st.v[r][2 * lane]);
+      rw[r] = ldraw(&st.w[r][2 * lane]);
     }
+    __syncwarp();
     if constexpr (SAVE8) {
-      float2 v[kRows], w[kRows];
+      if (z.rows > 0) {
+        float2 v[kRows], w[kRows];
 #pragma unroll
-      for (int r = 0; r < kRows; ++r) {
-        v[r] = value2(rv[r]);
-        w[r] = value2(rw[r]);
+        for (int r = 0; r < kRows; ++r) {
+          v[r] = value2(rv[r]);
+          w[r] = value2(rw[r]);
+        }
+        const float scale = put_int8(v, w, p.v8 + z.i + 2 * lane, p.w8 + z.i + 2 * lane, p.HD,
+                                     z.rows, lane);
+        if (lane < 2 * min(z.rows, kRows))
+          (lane & 1 ? p.ws : p.vs)[z.i / kGroup + (size_t)(lane >> 1) * groups] = scale;
       }
-      const float scale = put_int8(v, w, p.v8 + i0, p.w8 + i0, p.HD, rows, lane);
-      if (lane < 2 * rows)
-        (lane & 1 ? p.ws : p.vs)[(i0 - 2 * lane) / kGroup + (size_t)(lane >> 1) * groups] = scale;
     }
 #pragma unroll
     for (int r = 0; r < kRows; ++r) {
       a[r] = decay2<RAW>(value2(rg[r]));
       x[r] = mul2(gate2<RAW>(value2(rw[r])), value2(rv[r]));
     }
-  }
-  if (rows < kRows) {
+    if (z.rows < kRows) {
 #pragma unroll
-    for (int r = 0; r < kRows; ++r)
-      if (r >= rows) a[r] = both(1.f), x[r] = both(0.f);
-  }
-  Map m = {a[0], x[0]};
+      for (int r = 0; r < kRows; ++r)
+        if (r >= z.rows) a[r] = both(1.f), x[r] = both(0.f);
+    }
+    Map m = {a[0], x[0]};
 #pragma unroll
-  for (int r = 1; r < kRows; ++r) m = after({a[r], x[r]}, m);
-  map[warp][lane] = flat(m);
+    for (int r = 1; r < kRows; ++r) m = after({a[r], x[r]}, m);
+    map[warp][lane] = flat(m);
+  };
+
+  int now = tickets.first(p, joint.ticket);
+  if (!tickets.is(now)) return;
+  prefetch(now);
+  float2 a[kRows], x[kRows];
+  fold(now, a, x, maps[0]);
+  int next = tickets.second(p, joint.ticket + 1, now);
+  prefetch(next);
   __syncthreads();
-  float2 h = enter_tile(p, at, map, joint, p.h0);
-  if (warp == 0 && p.kept)
-    *reinterpret_cast<float2*>(p.kept + ((size_t)bb * p.tiles + at.k) * p.HD + ch) = h;
-  for (int j = 0; j < warp; ++j) h = apply(unflat(map[j][lane]), h);
-  float* o = p.o + i0;
+  if (warp == 1) publish_map(p, tickets.place(p, now), maps[0], lane);
+  for (int turn = 0; tickets.is(now); turn = turn == 2 ? 0 : turn + 1) {
+    const float4 (*map)[32] = maps[turn];
+    float4 (*coming)[32] = maps[turn == 2 ? 0 : turn + 1];
+    const Place at = tickets.place(p, now);
+    const Early early = look(p, at, warp, lane);
+    int later = tickets.total;
+    if (tickets.more) {
+      if (!tickets.drawn) later = next + (int)gridDim.x;
+      else if (threadIdx.x == 0) later = tickets.draw(p);
+    }
+    float2 na[kRows], nx[kRows];
+    const bool on = tickets.is(next);
+    if (on) fold(next, na, nx, coming);
+    __syncthreads();
+    if (warp == 1 && on) publish_map(p, tickets.place(p, next), coming, lane);
+    if (threadIdx.x == 0) joint.ticket[0] = later;
+    join(p, at, map, joint, p.h0, early, warp, lane);
+    __syncthreads();
+    if (tickets.drawn) later = joint.ticket[0];
+    prefetch(later);
+    const Rows z = rows_of(p, at, at.k, warp);
+    const int bb = at.chain / groups, ch = at.chain % groups * kGroup + 2 * lane;
+    float2 h = entering(joint, lane);
+    if (warp == 0 && p.kept)
+      *reinterpret_cast<float2*>(p.kept + ((size_t)bb * p.tiles + at.k) * p.HD + ch) = h;
+    h = walk(map, warp, lane, h);
+    float* o = p.o + z.i + 2 * lane;
 #pragma unroll
-  for (int r = 0; r < kRows; ++r) {
-    h = apply({a[r], x[r]}, h);
-    if (r < rows) st2(o + (size_t)r * p.HD, h);
+    for (int r = 0; r < kRows; ++r) {
+      h = apply({a[r], x[r]}, h);
+      if (r < z.rows) st2(o + (size_t)r * p.HD, h);
+    }
+    // rows behind the end keep the state
+    if (z.rows > 0 && z.rows <= kRows)
+      *reinterpret_cast<float2*>(p.hf + (size_t)bb * p.HD + ch) = h;
+#pragma unroll
+    for (int r = 0; r < kRows; ++r) {
+      a[r] = na[r];
+      x[r] = nx[r];
+    }
+    now = next;
+    next = later;
   }
-  // rows behind the end keep the state
-  if (rows > 0 && t0 + rows == p.T) *reinterpret_cast<float2*>(p.hf + (size_t)bb * p.HD + ch) = h;
 }
+
+// A few tokens (generation): a warp takes a chain alone, one token after another.
+// No maps, no shared memory; bound by the latency of one load and one store.
+constexpr int kStepTokens = 4;
+template <typename T, bool RAW>
+__global__ void __launch_bounds__(128) k_recur_step(const Args p) {
+  const int lane = threadIdx.x & 31, chain = blockIdx.x * 4 + (threadIdx.x >> 5);
+  if (chain >= p.chains) return;
+  const int groups = p.HD / kGroup, ch = chain % groups * kGroup + 2 * lane;
+  const size_t bb = chain / groups, i0 = bb * p.T * p.HD + ch, j = bb * p.HD + ch;
+  float2 h = p.h0 ? *reinterpret_cast<const float2*>(p.h0 + j) : both(0.f);
+  typename Raw<T>::type g[kStepTokens], v[kStepTokens], w[kStepTokens];
+#pragma unroll
+  for (int t = 0; t < kStepTokens; ++t) {
+    const size_t i = i0 + (size_t)min(t, p.T - 1) * p.HD;
+    g[t] = ldraw(static_cast<const T*>(p.g) + i);
+    v[t] = ldraw(static_cast<const T*>(p.v) + i);
+    w[t] = ldraw(static_cast<const T*>(p.w) + i);
+  }
+#pragma unroll
+  for (int t = 0; t < kStepTokens; ++t)
+    if (t < p.T) {
+      h = apply({decay2<RAW>(value2(g[t])), mul2(gate2<RAW>(value2(w[t])), value2(v[t]))}, h);
+      st2(p.o + i0 + (size_t)t * p.HD, h);
+    }
+  *reinterpret_cast<float2*>(p.hf + j) = h;
+}
+
+// The reverse scan needs g and dout alone until the state that enters a tile is
+// known; v and w come while the next tile is folded.
+template <typename T, typename V> struct BwdStage {
+  T g[kRows][kGroup];
+  float d[kRows][kGroup];
+  V v[kRows][kGroup], w[kRows][kGroup];
+  float scale[2 * kRows];   // of int8 v and w: 2 r + j of tensor j's row r
+};
 
 // Tiles in the order of the reverse scan: k = 0 is the last one in time, and the
 // maps of its warps are kept from the last warp to the first.
 template <typename T, bool FROM8, bool RAW>
-__global__ void __launch_bounds__(256) k_recur_bwd(const Args p) {
+__global__ void __launch_bounds__(256, 2) k_recur_bwd(const Args p) {
   using V = typename std::conditional<FROM8, int8_t, T>::type;
-  __shared__ float4 fmap[kWarps][32], rmap[kWarps][32];
+  extern __shared__ __align__(16) unsigned char raw_stage[];
+  __shared__ float4 maps[3][kWarps][32], fmap[kWarps][32];
   __shared__ Joint joint;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, back = kWarps - 1 - warp;
-  const Place at = take_tile(p);
-  const int groups = p.HD / kGroup, bb = at.chain / groups, cg = at.chain % groups;
-  const int tile = p.tiles - 1 - at.k;
-  const int ch = cg * kGroup + 2 * lane, t0 = tile * kTile + warp * kRows;
-  const int rows = min(kRows, p.T - t0);
-  const size_t i0 = ((size_t)bb * p.T + t0) * p.HD + ch;
-  float2 h = *reinterpret_cast<const float2*>(p.kept + ((size_t)bb * p.tiles + tile) * p.HD + ch);
-  float2 a[kRows], v[kRows], w[kRows], d[kRows];
-  if (rows > 0) {
-    typename Raw<T>::type rg[kRows];
-    typename Raw<V>::type rv[kRows], rw[kRows];
-    float scale = 0.f;   // lane 2 r + j: of tensor j's row r
+  BwdStage<T, V>& st = reinterpret_cast<BwdStage<T, V>*>(raw_stage)[warp];
+  const V* pv = FROM8 ? reinterpret_cast<const V*>(p.v8) : static_cast<const V*>(p.v);
+  const V* pw = FROM8 ? reinterpret_cast<const V*>(p.w8) : static_cast<const V*>(p.w);
+  const int groups = p.HD / kGroup;
+  const Tickets tickets(p);
+  auto prefetch = [&](int t) {
+    if (tickets.is(t)) {
+      const Place at = tickets.place(p, t);
+      const Rows z = rows_of(p, at, p.tiles - 1 - at.k, warp);
+      fetch(&st.g[0][0], static_cast<const T*>(p.g) + z.i, p.HD, z.rows, lane);
+      fetch(&st.d[0][0], p.dout + z.i, p.HD, z.rows, lane);
+    }
+    fetch_end();
+  };
+  auto prefetch_vw = [&](int t) {
+    if (tickets.is(t)) {
+      const Place at = tickets.place(p, t);
+      const Rows z = rows_of(p, at, p.tiles - 1 - at.k, warp);
+      fetch(&st.v[0][0], pv + z.i, p.HD, z.rows, lane);
+      fetch(&st.w[0][0], pw + z.i, p.HD, z.rows, lane);
+      if (FROM8 && lane < 2 * min(z.rows, kRows))
+        fetch4(&st.scale[lane], (lane & 1 ? p.ws : p.vs) + z.i / kGroup + (size_t)(lane >> 1) * groups);
+    }
+    fetch_end();
+  };
+  // decays and cotangents of tile t, and the warp's map of the reverse scan
+  auto fold = [&](int t, float2 (&a)[kRows], float2 (&d)[kRows], float4 (*map)[32]) {
+    const Place at = tickets.place(p, t);
+    const Rows z = rows_of(p, at, p.tiles - 1 - at.k, warp);
+    fetched<1>();
 #pragma unroll
     for (int r = 0; r < kRows; ++r) {
-      const size_t i = i0 + (size_t)min(r, rows - 1) * p.HD;
-      rv[r] = ldraw((FROM8 ? reinterpret_cast<const V*>(p.v8) : static_cast<const V*>(p.v)) + i);
-      rw[r] = ldraw((FROM8 ? reinterpret_cast<const V*>(p.w8) : static_cast<const V*>(p.w)) + i);
-      rg[r] = ldraw(static_cast<const T*>(p.g) + i);
-      d[r] = ldraw(p.dout + i);
+      a[r] = value2(ldraw(&st.g[r][2 * lane]));
+      d[r] = ldraw(&st.d[r][2 * lane]);
     }
-    if (FROM8 && lane < 2 * rows)
-      scale = (lane & 1 ? p.ws : p.vs)[(i0 - 2 * lane) / kGroup + (size_t)(lane >> 1) * groups];
+    __syncwarp();
 #pragma unroll
-    for (int r = 0; r < kRows; ++r) {
-      v[r] = value2(rv[r]);
-      w[r] = value2(rw[r]);
-      if constexpr (FROM8) {
-        v[r] = mul2(v[r], both(__shfl_sync(0xffffffffu, scale, 2 * r)));
-        w[r] = mul2(w[r], both(__shfl_sync(0xffffffffu, scale, 2 * r + 1)));
-      }
-      w[r] = gate2<RAW>(w[r]);
-      a[r] = decay2<RAW>(value2(rg[r]));
+    for (int r = 0; r < kRows; ++r) a[r] = decay2<RAW>(a[r]);
+    if (z.rows < kRows) {
+#pragma unroll
+      for (int r = 0; r < kRows; ++r)
+        if (r >= z.rows) a[r] = both(1.f), d[r] = both(0.f);
     }
-  }
-  if (rows < kRows) {   // the identity, in both directions
+    Map m = identity();
 #pragma unroll
-    for (int r = 0; r < kRows; ++r)
-      if (r >= rows) a[r] = both(1.f), v[r] = w[r] = d[r] = both(0.f);
-  }
-  Map m = {a[0], mul2(w[0], v[0])}, n = identity();
-#pragma unroll
-  for (int r = 1; r < kRows; ++r) m = after({a[r], mul2(w[r], v[r])}, m);
-#pragma unroll
-  for (int r = kRows - 1; r >= 0; --r) n.b = mul2(a[r], add2(d[r], n.b));
-  n.a = m.a;
-  fmap[warp][lane] = flat(m);
-  rmap[back][lane] = flat(n);
+    for (int r = kRows - 1; r >= 0; --r) m = {mul2(a[r], m.a), mul2(a[r], add2(d[r], m.b))};
+    map[back][lane] = flat(m);
+  };
+  // v and w of row r of the present tile
+  auto vw = [&](int r, int rows, float2& v, float2& w) {
+    v = value2(ldraw(&st.v[r][2 * lane]));
+    w = value2(ldraw(&st.w[r][2 * lane]));
+    if constexpr (FROM8) {
+      v = mul2(v, both(st.scale[2 * r]));
+      w = mul2(w, both(st.scale[2 * r + 1]));
+    }
+    w = gate2<RAW>(w);
+    if (r >= rows) v = w = both(0.f);
+  };
+
+  int now = tickets.first(p, joint.ticket);
+  if (!tickets.is(now)) return;
+  prefetch(now);
+  prefetch_vw(now);
+  float2 a[kRows], d[kRows];
+  fold(now, a, d, maps[0]);
+  int next = tickets.second(p, joint.ticket + 1, now);
+  prefetch(next);
   __syncthreads();
-  float2 c = enter_tile(p, at, rmap, joint, p.dhf);
-  for (int j = 0; j < warp; ++j) h = apply(unflat(fmap[j][lane]), h);
-  for (int j = 0; j < back; ++j) c = apply(unflat(rmap[j][lane]), c);
-  float2 before[kRows];
-#pragma unroll
-  for (int r = 0; r < kRows; ++r) {
-    before[r] = h;
-    h = apply({a[r], mul2(w[r], v[r])}, h);
-  }
-#pragma unroll
-  for (int r = kRows - 1; r >= 0; --r) {
-    const float2 dh = add2(d[r], c);
-    c = mul2(a[r], dh);
-    if (r < rows) {
-      const size_t i = i0 + (size_t)r * p.HD;
-      float2 dw = mul2(v[r], dh), dg = mul2(before[r], c);
-      if constexpr (RAW) {
-        // d sigmoid(x) = w (1 - w); dg/dx = -sigmoid(x)
-        dw = make_float2(dw.x * (w[r].x * (1.f - w[r].x)), dw.y * (w[r].y * (1.f - w[r].y)));
-        const float2 g = value2(ldraw(static_cast<const T*>(p.g) + i));   // in L2
-        dg = make_float2(-dg.x * sig(g.x), -dg.y * sig(g.y));
-      }
-      st2(static_cast<T*>(p.dv) + i, mul2(w[r], dh));
-      st2(static_cast<T*>(p.dw) + i, dw);
-      st2(static_cast<T*>(p.dg) + i, dg);
+  if (warp == 1) publish_map(p, tickets.place(p, now), maps[0], lane);
+  // in flight here and at the end of each turn: v, w of `now` and g, dout of
+  // `next`, the one that is needed first first
+  for (int turn = 0, begin = 1; tickets.is(now); turn = turn == 2 ? 0 : turn + 1, begin = 0) {
+    const float4 (*map)[32] = maps[turn];
+    float4 (*coming)[32] = maps[turn == 2 ? 0 : turn + 1];
+    const Place at = tickets.place(p, now);
+    const int tile = p.tiles - 1 - at.k;
+    const Rows z = rows_of(p, at, tile, warp);
+    const int bb = at.chain / groups, ch = at.chain % groups * kGroup + 2 * lane;
+    const Early early = look(p, at, warp, lane);
+    float2 h = *reinterpret_cast<const float2*>(p.kept + ((size_t)bb * p.tiles + tile) * p.HD + ch);
+    int later = tickets.total;
+    if (tickets.more) {
+      if (!tickets.drawn) later = next + (int)gridDim.x;
+      else if (threadIdx.x == 0) later = tickets.draw(p);
     }
+    float2 na[kRows], nd[kRows];
+    const bool on = tickets.is(next);
+    if (begin) fetched<0>();
+    if (on) fold(next, na, nd, coming);
+    fetched<0>();
+    Map m = identity();
+#pragma unroll
+    for (int r = 0; r < kRows; ++r) {
+      float2 v, w;
+      vw(r, z.rows, v, w);
+      m = after({a[r], mul2(w, v)}, m);
+    }
+    __syncthreads();
+    if (warp == 1 && on) publish_map(p, tickets.place(p, next), coming, lane);
+    if (threadIdx.x == 0) joint.ticket[0] = later;
+    fmap[warp][lane] = flat(m);
+    join(p, at, map, joint, p.dhf, early, warp, lane);
+    __syncthreads();
+    if (tickets.drawn) later = joint.ticket[0];
+    prefetch(later);
+    h = walk(fmap, warp, lane, h);
+    float2 c = walk(map, back, lane, entering(joint, lane));
+    float2 before[kRows];
+#pragma unroll
+    for (int r = 0; r < kRows; ++r) {
+      float2 v, w;
+      vw(r, z.rows, v, w);
+      before[r] = h;
+      h = apply({a[r], mul2(w, v)}, h);
+    }
+#pragma unroll
+    for (int r = kRows - 1; r >= 0; --r) {
+      const float2 dh = add2(d[r], c);
+      c = mul2(a[r], dh);
+      if (r < z.rows) {
+        const size_t i = z.i + 2 * lane + (size_t)r * p.HD;
+        float2 v, w;
+        vw(r, kRows, v, w);
+        float2 dw = mul2(v, dh), dg = mul2(before[r], c);
+        if constexpr (RAW) {
+          // d sigmoid(x) = w (1 - w); dg/dx = -sigmoid(x)
+          dw = make_float2(dw.x * (w.x * (1.f - w.x)), dw.y * (w.y * (1.f - w.y)));
+          const float2 g = value2(ldraw(static_cast<const T*>(p.g) + i));   // in L2
+          dg = make_float2(-dg.x * sig(g.x), -dg.y * sig(g.y));
+        }
+        st2(static_cast<T*>(p.dv) + i, mul2(w, dh));
+        st2(static_cast<T*>(p.dw) + i, dw);
+        st2(static_cast<T*>(p.dg) + i, dg);
+      }
+    }
+    if (tile == 0 && warp == 0) *reinterpret_cast<float2*>(p.dh0 + (size_t)bb * p.HD + ch) = c;
+    __syncwarp();
+    prefetch_vw(next);
+#pragma unroll
+    for (int r = 0; r < kRows; ++r) {
+      a[r] = na[r];
+      d[r] = nd[r];
+    }
+    now = next;
+    next = later;
   }
-  if (tile == 0 && warp == 0) *reinterpret_cast<float2*>(p.dh0 + (size_t)bb * p.HD + ch) = c;
 }
 
+// One CTA for every place on the GPU, or one a tile where there are fewer.
+template <typename K>
+cudaError_t launch_tiles(K kernel, size_t stage, int per_sm, const Args& p, cudaStream_t s) {
+  int dev = 0, sms = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e == cudaSuccess) e = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
+  if (e == cudaSuccess)
+    e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)stage);
+  if (e != cudaSuccess) return e;
+  const size_t tiles = (size_t)p.chains * p.tiles, places = (size_t)sms * per_sm;
+  kernel<<<(unsigned)(tiles < places ? tiles : places), 256, stage, s>>>(p);
+  return cudaGetLastError();
+}
 template <bool FWD, typename T>
-void launch(const Args& p, bool int8, bool raw, cudaStream_t s) {
-  const unsigned grid = (unsigned)((size_t)p.chains * p.tiles);
-  auto go = [&](auto kernel) { kernel<<<grid, 256, 0, s>>>(p); };
+cudaError_t launch(const Args& p, bool int8, bool raw, cudaStream_t s) {
   if constexpr (FWD) {
-    if (int8) raw ? go(k_recur_fwd<T, true, true>) : go(k_recur_fwd<T, true, false>);
-    else raw ? go(k_recur_fwd<T, false, true>) : go(k_recur_fwd<T, false, false>);
+    // 4 tokens: the serial walk costs what a tile's joins do
+    if (p.T <= kStepTokens && !int8 && !p.kept) {
+      const unsigned grid = (unsigned)((p.chains + 3) / 4);
+      if (raw) k_recur_step<T, true><<<grid, 128, 0, s>>>(p);
+      else k_recur_step<T, false><<<grid, 128, 0, s>>>(p);
+      return cudaGetLastError();
+    }
+    auto go = [&](auto kernel) { return launch_tiles(kernel, sizeof(FwdStage<T>) * kWarps, 2, p, s); };
+    if (int8) return raw ? go(k_recur_fwd<T, true, true>) : go(k_recur_fwd<T, true, false>);
+    return raw ? go(k_recur_fwd<T, false, true>) : go(k_recur_fwd<T, false, false>);
   } else {
-    if (int8) raw ? go(k_recur_bwd<T, true, true>) : go(k_recur_bwd<T, true, false>);
-    else raw ? go(k_recur_bwd<T, false, true>) : go(k_recur_bwd<T, false, false>);
+    auto go = [&](auto kernel, size_t stage) { return launch_tiles(kernel, stage * kWarps, 2, p, s); };
+    const size_t n = sizeof(BwdStage<T, T>), n8 = sizeof(BwdStage<T, int8_t>);
+    if (int8) return raw ? go(k_recur_bwd<T, true, true>, n8) : go(k_recur_bwd<T, true, false>, n8);
+    return raw ? go(k_recur_bwd<T, false, true>, n) : go(k_recur_bwd<T, false, false>, n);
   }
 }
 
@@ -413,7 +682,7 @@ int check(int dtype, int B, int T, int H, int D) {
     return report_error(GDN2_ERR_INVALID, "gdn2_recur: head dim D unsupported (64, 128 or 256)");
   const long chains = (long)B * ((long)H * (D / kGroup));
   if (T > (1 << 30) || (long)H * D > (1 << 24) || chains > (1 << 26) ||
-      chains * ((T + kTile - 1) / kTile) > 0x7fffffffL)
+      chains * ((T + kTile - 1) / kTile) > (1L << 30))   // tickets stay in 31 bits
     return report_error(GDN2_ERR_INVALID, "gdn2_recur: too many tokens or channels");
   return GDN2_OK;
 }
@@ -433,8 +702,7 @@ int prepare(Args& p, int B, void* workspace, cudaStream_t s) {
   return e == cudaSuccess ? GDN2_OK : report_error(GDN2_ERR_CUDA, cudaGetErrorString(e));
 }
 
-int launched() {
-  const cudaError_t e = cudaGetLastError();
+int launched(cudaError_t e) {
   return e == cudaSuccess ? GDN2_OK : report_error(GDN2_ERR_CUDA, cudaGetErrorString(e));
 }
 
@@ -474,9 +742,8 @@ extern "C" int gdn2_recur_fwd(int dtype, const void* v, const void* w, const voi
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   const int e = prepare(p, B, workspace, s);
   if (e) return e;
-  if (dtype == GDN2_F32) launch<true, float>(p, save8, raw, s);
-  else launch<true, __nv_bfloat16>(p, save8, raw, s);
-  return launched();
+  return launched(dtype == GDN2_F32 ? launch<true, float>(p, save8, raw, s)
+                                    : launch<true, __nv_bfloat16>(p, save8, raw, s));
 }
 
 extern "C" int gdn2_recur_bwd(int dtype, const void* v, const void* w, const void* g,
@@ -511,7 +778,6 @@ extern "C" int gdn2_recur_bwd(int dtype, const void* v, const void* w, const voi
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   const int e = prepare(p, B, workspace, s);
   if (e) return e;
-  if (dtype == GDN2_F32) launch<false, float>(p, from8, raw, s);
-  else launch<false, __nv_bfloat16>(p, from8, raw, s);
-  return launched();
+  return launched(dtype == GDN2_F32 ? launch<false, float>(p, from8, raw, s)
+                                    : launch<false, __nv_bfloat16>(p, from8, raw, s));
 }
