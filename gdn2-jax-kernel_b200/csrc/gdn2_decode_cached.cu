@@ -25,7 +25,7 @@ int report_error(int code, const char* msg);
 namespace {
 
 #ifndef MINB
-#define MINB 3
+#define MINB 4
 #endif
 template <int D> struct Shape {
   static constexpr int NW = D / 16;          // warps

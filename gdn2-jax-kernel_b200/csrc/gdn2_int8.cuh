@@ -5,8 +5,8 @@
 // The code is the correctly rounded one: it does not depend on the order or
 // the precision of the arithmetic that a caller compares with.  The error of a
 // value is at most half a step, max|x| / 254.
-//   * A group whose largest |x| is below 2^-100 is stored as zeros (its scale
-//     would leave the normal range).
+//   * A group whose largest |x| is below 2^-100 gets the scale 0 and reads back as
+//     zeros (its scale would leave the normal range).
 //   * A group that holds a NaN or an infinity gets a NaN scale, so all of it
 //     reads back as NaN: one scale cannot hold an infinity next to other values,
 //     and a silent 0 would hide it.
@@ -68,12 +68,13 @@ __device__ __forceinline__ float max_abs3(float x, float y, float z) {
   return r;
 }
 
-// 127 / top for the codes, to 2^-22.5 of itself (what that leaves open,
-// int8_code4 decides); 0, so that every code is 0, for a group without a scale.
+// 127 / top for the codes, to 2^-22.5 of itself (what that leaves open the border
+// check decides).  Finite for every top: a group without a scale reads back as 0
+// or NaN whatever its codes.
 __device__ __forceinline__ float group_inv(float top) {
   float r;
-  asm("rcp.approx.f32 %0, %1;" : "=f"(r) : "f"(top));
-  return top >= kInt8Tiny && top <= 3.402823466e38f ? 127.f * r : 0.f;
+  asm("rcp.approx.f32 %0, %1;" : "=f"(r) : "f"(fmaxf(top, kInt8Tiny)));
+  return 127.f * r;
 }
 // The stored scale, rounded once.
 __device__ __forceinline__ float group_scale(float top) {
@@ -88,32 +89,51 @@ static __device__ __noinline__ float int8_border(float x, float y, float top) {
   const bool up = l > r || (l == r && ((int)lo & 1));
   return copysignf(lo + (up ? 1.f : 0.f), x);
 }
-// The codes of N values of one group, each in the low byte of a word.
+// The codes of N (even) values of one group, each in the low byte of a word.
 // kCodeBias added to y = x * inv, |y| <= 127.01, rounds it to a whole number in the
 // low bits (the conversion and rounding instructions run at an eighth of the
 // rate).  y is off by at most 127 * 2^-22.5 = 2.2e-5, so only a y within 1e-4 of
 // a half can round the wrong way: one value in 5000 is decided in float64.
 template <int N>
-__device__ __forceinline__ void int8_codes(const float (&x)[N], float inv, float top,
-                                           unsigned (&code)[N]) {
-  float far = 0.f;
+__device__ __forceinline__ float int8_near(const float (&x)[N], float inv, unsigned (&code)[N]) {
+  float far = 0.f;   // the largest distance of a y from its code
+#pragma unroll
+  for (int i = 0; i < N; i += 2) {
+    const float2 v = make_float2(x[i], x[i + 1]), t = fma2(v, both(inv), both(kCodeBias));
+    const float2 r = fma2(v, both(inv), fma2(t, both(-1.f), both(kCodeBias)));
+    far = fmaxf(far, fmaxf(fabsf(r.x), fabsf(r.y)));
+    code[i] = __float_as_uint(t.x);
+    code[i + 1] = __float_as_uint(t.y);
+  }
+  return far;
+}
+template <int N>
+__device__ __forceinline__ void int8_decide(const float (&x)[N], float inv, float top, unsigned (&code)[N]) {
 #pragma unroll
   for (int i = 0; i < N; ++i) {
-    const float t = fmaf(x[i], inv, kCodeBias);
-    far = fmaxf(far, fabsf(fmaf(x[i], inv, kCodeBias - t)));
-    code[i] = __float_as_uint(t);
+    const float y = x[i] * inv, r = __uint_as_float(code[i]) - kCodeBias;
+    if (fabsf(y - r) > 0.4998f)
+      code[i] = __float_as_uint(int8_border(x[i], y, top) + kCodeBias);
   }
-  if (far > 0.4999f) {
-#pragma unroll
-    for (int i = 0; i < N; ++i) {
-      const float y = x[i] * inv, r = __uint_as_float(code[i]) - kCodeBias;
-      if (fabsf(y - r) > 0.4998f)
-        code[i] = __float_as_uint(int8_border(x[i], y, top) + kCodeBias);
-    }
-  }
+}
+template <int N>
+__device__ __forceinline__ void int8_codes(const float (&x)[N], float inv, float top,
+                                           unsigned (&code)[N]) {
+  if (int8_near(x, inv, code) > 0.4999f) int8_decide(x, inv, top, code);
 }
 __device__ __forceinline__ unsigned pack4(unsigned a, unsigned b, unsigned c, unsigned d) {
   return __byte_perm(__byte_perm(a, b, 0x0040), __byte_perm(c, d, 0x0040), 0x5410);
+}
+// Two values each of two groups: the four codes as bytes.
+__device__ __forceinline__ unsigned int8_codes2x2(float2 v, float2 w, float tv, float tw) {
+  const float x[2] = {v.x, v.y}, y[2] = {w.x, w.y}, iv = group_inv(tv), iw = group_inv(tw);
+  unsigned c[2], d[2];
+  const float far = int8_near(x, iv, c);
+  if (fmaxf(far, int8_near(y, iw, d)) > 0.4999f) {
+    int8_decide(x, iv, tv, c);
+    int8_decide(y, iw, tw, d);
+  }
+  return pack4(c[0], c[1], d[0], d[1]);
 }
 // Byte I of four codes as a float: the code moved to 0..255 becomes the low
 // byte of 2^23 + code, and one exact subtraction takes both offsets off (the

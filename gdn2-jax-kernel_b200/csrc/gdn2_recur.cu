@@ -105,13 +105,30 @@ __device__ __forceinline__ void st2(__nv_bfloat16* p, float2 v) {
   __stcs(reinterpret_cast<unsigned*>(p), *reinterpret_cast<const unsigned*>(&h));
 }
 
-// e^g, or from the pre-activation x of g = -softplus(x): sigmoid(-x), from
-// e^{-|x|} so that neither end overflows or cancels.
-__device__ __forceinline__ float sig_from(float e, bool high) { return (high ? 1.f : e) / (1.f + e); }
-__device__ __forceinline__ float sig(float x) { return sig_from(expf(-fabsf(x)), x > 0.f); }
+// e^g as 2^(g log2 e): off by 2^-22 + |g| 2^-23 of itself (0 below 2^-126).  The
+// part that grows with |g| does not add up over a sequence: after decays that
+// sum to S a term has the weight e^-S, and S e^-S 2^-23 is at most 2^-24.4 of it
+// where expf took 16 of the 40 instructions of a row.
+__device__ __forceinline__ float ex2(float x) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+constexpr float kLog2e = 1.4426950408889634f;
+// sigmoid(x) from e^{-|x|}, so that neither end overflows or cancels; subnormal
+// values stay (the gradient of a gate that is nearly shut).
+__device__ __forceinline__ float sig(float x) {
+  float e, r;
+  asm("ex2.approx.f32 %0, %1;" : "=f"(e) : "f"(-kLog2e * fabsf(x)));
+  asm("rcp.approx.f32 %0, %1;" : "=f"(r) : "f"(1.f + e));
+  return x > 0.f ? r : e * r;
+}
+// e^g, or from the pre-activation x of g = -softplus(x): sigmoid(-x).
 template <bool RAW>
 __device__ __forceinline__ float2 decay2(float2 g) {
-  return RAW ? make_float2(sig(-g.x), sig(-g.y)) : make_float2(expf(g.x), expf(g.y));
+  if constexpr (RAW) return make_float2(sig(-g.x), sig(-g.y));
+  const float2 t = mul2(g, both(kLog2e));
+  return make_float2(ex2(t.x), ex2(t.y));
 }
 template <bool RAW>
 __device__ __forceinline__ float2 gate2(float2 w) {
@@ -184,44 +201,38 @@ struct Args {
 };
 
 // Tiles are taken in the order of time: ticket t is tile t / chains of chain
-// t % chains, in the order of the scan.  A CTA holds the tile it works on and the
-// next one, whose bytes are on their way meanwhile; what a tile waits for has a
-// lower ticket, and the lowest unfinished ticket is always being worked on.
-// Sequences of one tile wait for nothing and are dealt out by index.
-struct Place { int chain, k; };
+// t % chains, in the order of the scan.  A CTA holds the tile it works on, the
+// next one and the one after; what a tile waits for has a lower ticket, and the
+// lowest unfinished ticket is always being worked on.  Sequences of one tile
+// wait for nothing and are dealt out by index.
+// A ticket is taken apart by one thread for all (four divisions a warp for every
+// tile cost a third of the instructions).
+struct Place { int k, chain, bb, cg; };   // k < 0: none left
 struct Tickets {
-  int total;
   bool drawn, more;   // from the counter; more than one a CTA
+  int total, mine;    // mine: of thread 0, the latest
   __device__ __forceinline__ Tickets(const Args& p)
-      : total(p.tiles * p.chains), drawn(p.tiles > 1), more(total > (int)gridDim.x) {}
-  __device__ __forceinline__ int draw(const Args& p) const { return atomicAdd(p.s.status + 8, 1); }
-  __device__ __forceinline__ int first(const Args& p, int* shared) const {
-    if (!drawn) return blockIdx.x;
-    if (threadIdx.x == 0) *shared = draw(p);
-    __syncthreads();
-    return *shared;
+      : drawn(p.tiles > 1), more(p.tiles * p.chains > (int)gridDim.x), total(p.tiles * p.chains), mine(0) {}
+  // thread 0: asks for a ticket, then takes it apart
+  __device__ __forceinline__ void ask(const Args& p, bool first) {
+    if (!first && !more) mine = total;
+    else if (drawn) mine = atomicAdd(p.s.status + 8, 1);
+    else mine = first ? (int)blockIdx.x : mine + (int)gridDim.x;
   }
-  // Drawn once the first tile's bytes are there, when other CTAs have theirs:
-  // one that drew two at once would leave another without any.
-  __device__ __forceinline__ int second(const Args& p, int* shared, int now) const {
-    if (!more) return total;
-    if (!drawn) return now + gridDim.x;
-    if (threadIdx.x == 0) *shared = draw(p);
-    __syncthreads();
-    return *shared;
-  }
-  __device__ __forceinline__ bool is(int t) const { return t < total; }
-  __device__ __forceinline__ Place place(const Args& p, int t) const {
-    return {(int)((unsigned)t % p.chains), (int)((unsigned)t / p.chains)};
+  __device__ __forceinline__ int4 place(const Args& p) const {
+    if (mine >= total) return make_int4(-1, 0, 0, 0);
+    const unsigned chain = (unsigned)mine % p.chains, groups = p.HD / kGroup;
+    return make_int4((unsigned)mine / p.chains, chain, chain / groups, chain % groups);
   }
 };
+__device__ __forceinline__ Place told(const int4& z) { return {z.x, z.y, z.z, z.w}; }
 
 // How a tile of a chain gets the state that enters it (map: the maps of its warps
 // in the order of the scan).
 struct Joint {
   float4 pairs[kWarps][32];   // the mates 2 w and 2 w + 1 before it in its group
   float2 enter[32];           // the state that enters the group
-  int ticket[2];
+  int4 place[2];
 };
 __device__ __forceinline__ ulonglong2* map_of(const Args& p, Place at, int k, int lane) {
   return p.s.maps + ((size_t)k * p.chains + at.chain) * 32 + lane;
@@ -306,12 +317,10 @@ __device__ __forceinline__ float put_int8(const float2 (&v)[kRows], const float2
   for (int r = 0; r < kRows; ++r) {
     const float tv = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(max_abs(v[r].x, v[r].y))));
     const float tw = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(max_abs(w[r].x, w[r].y))));
-    unsigned c[2], d[2];
-    int8_codes<2>({v[r].x, v[r].y}, group_inv(tv), tv, c);
-    int8_codes<2>({w[r].x, w[r].y}, group_inv(tw), tw, d);
+    const unsigned c = int8_codes2x2(v[r], w[r], tv, tw);
     if (r < rows) {
-      *reinterpret_cast<unsigned short*>(v8 + r * stride) = (unsigned short)__byte_perm(c[0], c[1], 0x0040);
-      *reinterpret_cast<unsigned short*>(w8 + r * stride) = (unsigned short)__byte_perm(d[0], d[1], 0x0040);
+      *reinterpret_cast<unsigned short*>(v8 + r * stride) = (unsigned short)c;
+      *reinterpret_cast<unsigned short*>(w8 + r * stride) = (unsigned short)(c >> 16);
     }
     mine = lane == 2 * r ? tv : lane == 2 * r + 1 ? tw : mine;
   }
@@ -319,11 +328,10 @@ __device__ __forceinline__ float put_int8(const float2 (&v)[kRows], const float2
 }
 
 // Where a tile lies for a warp: rows of it (8 and more: all eight), first element.
-struct Rows { int t0, rows; size_t i; };
+struct Rows { int rows; size_t i; };
 __device__ __forceinline__ Rows rows_of(const Args& p, Place at, int tile, int warp) {
-  const int groups = p.HD / kGroup, t0 = tile * kTile + warp * kRows;
-  return {t0, p.T - t0,
-          ((size_t)(at.chain / groups) * p.T + t0) * p.HD + at.chain % groups * kGroup};
+  const int t0 = tile * kTile + warp * kRows;
+  return {p.T - t0, ((size_t)at.bb * p.T + t0) * p.HD + at.cg * kGroup};
 }
 
 // Shared memory of a warp: its 8 rows of the tile that comes next.
@@ -337,10 +345,9 @@ __global__ void __launch_bounds__(256, 2) k_recur_fwd(const Args p) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   FwdStage<T>& st = reinterpret_cast<FwdStage<T>*>(raw_stage)[warp];
   const int groups = p.HD / kGroup;
-  const Tickets tickets(p);
-  auto prefetch = [&](int t) {
-    if (tickets.is(t)) {
-      const Place at = tickets.place(p, t);
+  Tickets tickets(p);
+  auto prefetch = [&](Place at) {
+    if (at.k >= 0) {
       const Rows z = rows_of(p, at, at.k, warp);
       fetch(&st.g[0][0], static_cast<const T*>(p.g) + z.i, p.HD, z.rows, lane);
       fetch(&st.v[0][0], static_cast<const T*>(p.v) + z.i, p.HD, z.rows, lane);
@@ -349,8 +356,7 @@ __global__ void __launch_bounds__(256, 2) k_recur_fwd(const Args p) {
     fetch_end();
   };
   // the rows of tile t as maps (a, x), and the map of the warp
-  auto fold = [&](int t, float2 (&a)[kRows], float2 (&x)[kRows], float4 (*map)[32]) {
-    const Place at = tickets.place(p, t);
+  auto fold = [&](Place at, float2 (&a)[kRows], float2 (&x)[kRows], float4 (*map)[32]) {
     const Rows z = rows_of(p, at, at.k, warp);
     typename Raw<T>::type rg[kRows], rv[kRows], rw[kRows];
     fetched<0>();
@@ -391,37 +397,44 @@ __global__ void __launch_bounds__(256, 2) k_recur_fwd(const Args p) {
     map[warp][lane] = flat(m);
   };
 
-  int now = tickets.first(p, joint.ticket);
-  if (!tickets.is(now)) return;
+  if (threadIdx.x == 0) {
+    tickets.ask(p, true);
+    joint.place[0] = tickets.place(p);
+  }
+  __syncthreads();
+  Place now = told(joint.place[0]);
+  if (now.k < 0) return;
   prefetch(now);
   float2 a[kRows], x[kRows];
   fold(now, a, x, maps[0]);
-  int next = tickets.second(p, joint.ticket + 1, now);
-  prefetch(next);
+  // the second ticket once the first tile's bytes are there, when other CTAs have
+  // theirs: one that drew two at once would leave another without any
+  if (threadIdx.x == 0) {
+    tickets.ask(p, false);
+    joint.place[1] = tickets.place(p);
+  }
   __syncthreads();
-  if (warp == 1) publish_map(p, tickets.place(p, now), maps[0], lane);
-  for (int turn = 0; tickets.is(now); turn = turn == 2 ? 0 : turn + 1) {
+  Place next = told(joint.place[1]);
+  prefetch(next);
+  if (warp == 1) publish_map(p, now, maps[0], lane);
+  for (int turn = 0; now.k >= 0; turn = turn == 2 ? 0 : turn + 1) {
     const float4 (*map)[32] = maps[turn];
     float4 (*coming)[32] = maps[turn == 2 ? 0 : turn + 1];
-    const Place at = tickets.place(p, now);
+    const Place at = now;
     const Early early = look(p, at, warp, lane);
-    int later = tickets.total;
-    if (tickets.more) {
-      if (!tickets.drawn) later = next + (int)gridDim.x;
-      else if (threadIdx.x == 0) later = tickets.draw(p);
-    }
+    if (threadIdx.x == 0) tickets.ask(p, false);
     float2 na[kRows], nx[kRows];
-    const bool on = tickets.is(next);
+    const bool on = next.k >= 0;
     if (on) fold(next, na, nx, coming);
     __syncthreads();
-    if (warp == 1 && on) publish_map(p, tickets.place(p, next), coming, lane);
-    if (threadIdx.x == 0) joint.ticket[0] = later;
+    if (warp == 1 && on) publish_map(p, next, coming, lane);
+    if (threadIdx.x == 0) joint.place[0] = tickets.place(p);
     join(p, at, map, joint, p.h0, early, warp, lane);
     __syncthreads();
-    if (tickets.drawn) later = joint.ticket[0];
+    const Place later = told(joint.place[0]);
     prefetch(later);
     const Rows z = rows_of(p, at, at.k, warp);
-    const int bb = at.chain / groups, ch = at.chain % groups * kGroup + 2 * lane;
+    const int bb = at.bb, ch = at.cg * kGroup + 2 * lane;
     float2 h = entering(joint, lane);
     if (warp == 0 && p.kept)
       *reinterpret_cast<float2*>(p.kept + ((size_t)bb * p.tiles + at.k) * p.HD + ch) = h;
@@ -494,19 +507,17 @@ __global__ void __launch_bounds__(256, 2) k_recur_bwd(const Args p) {
   const V* pv = FROM8 ? reinterpret_cast<const V*>(p.v8) : static_cast<const V*>(p.v);
   const V* pw = FROM8 ? reinterpret_cast<const V*>(p.w8) : static_cast<const V*>(p.w);
   const int groups = p.HD / kGroup;
-  const Tickets tickets(p);
-  auto prefetch = [&](int t) {
-    if (tickets.is(t)) {
-      const Place at = tickets.place(p, t);
+  Tickets tickets(p);
+  auto prefetch = [&](Place at) {
+    if (at.k >= 0) {
       const Rows z = rows_of(p, at, p.tiles - 1 - at.k, warp);
       fetch(&st.g[0][0], static_cast<const T*>(p.g) + z.i, p.HD, z.rows, lane);
       fetch(&st.d[0][0], p.dout + z.i, p.HD, z.rows, lane);
     }
     fetch_end();
   };
-  auto prefetch_vw = [&](int t) {
-    if (tickets.is(t)) {
-      const Place at = tickets.place(p, t);
+  auto prefetch_vw = [&](Place at) {
+    if (at.k >= 0) {
       const Rows z = rows_of(p, at, p.tiles - 1 - at.k, warp);
       fetch(&st.v[0][0], pv + z.i, p.HD, z.rows, lane);
       fetch(&st.w[0][0], pw + z.i, p.HD, z.rows, lane);
@@ -516,8 +527,7 @@ __global__ void __launch_bounds__(256, 2) k_recur_bwd(const Args p) {
     fetch_end();
   };
   // decays and cotangents of tile t, and the warp's map of the reverse scan
-  auto fold = [&](int t, float2 (&a)[kRows], float2 (&d)[kRows], float4 (*map)[32]) {
-    const Place at = tickets.place(p, t);
+  auto fold = [&](Place at, float2 (&a)[kRows], float2 (&d)[kRows], float4 (*map)[32]) {
     const Rows z = rows_of(p, at, p.tiles - 1 - at.k, warp);
     fetched<1>();
 #pragma unroll
@@ -550,34 +560,41 @@ __global__ void __launch_bounds__(256, 2) k_recur_bwd(const Args p) {
     if (r >= rows) v = w = both(0.f);
   };
 
-  int now = tickets.first(p, joint.ticket);
-  if (!tickets.is(now)) return;
+  if (threadIdx.x == 0) {
+    tickets.ask(p, true);
+    joint.place[0] = tickets.place(p);
+  }
+  __syncthreads();
+  Place now = told(joint.place[0]);
+  if (now.k < 0) return;
   prefetch(now);
   prefetch_vw(now);
   float2 a[kRows], d[kRows];
   fold(now, a, d, maps[0]);
-  int next = tickets.second(p, joint.ticket + 1, now);
-  prefetch(next);
+  // the second ticket once the first tile's bytes are there, when other CTAs have
+  // theirs: one that drew two at once would leave another without any
+  if (threadIdx.x == 0) {
+    tickets.ask(p, false);
+    joint.place[1] = tickets.place(p);
+  }
   __syncthreads();
-  if (warp == 1) publish_map(p, tickets.place(p, now), maps[0], lane);
+  Place next = told(joint.place[1]);
+  prefetch(next);
+  if (warp == 1) publish_map(p, now, maps[0], lane);
   // in flight here and at the end of each turn: v, w of `now` and g, dout of
   // `next`, the one that is needed first first
-  for (int turn = 0, begin = 1; tickets.is(now); turn = turn == 2 ? 0 : turn + 1, begin = 0) {
+  for (int turn = 0, begin = 1; now.k >= 0; turn = turn == 2 ? 0 : turn + 1, begin = 0) {
     const float4 (*map)[32] = maps[turn];
     float4 (*coming)[32] = maps[turn == 2 ? 0 : turn + 1];
-    const Place at = tickets.place(p, now);
+    const Place at = now;
     const int tile = p.tiles - 1 - at.k;
     const Rows z = rows_of(p, at, tile, warp);
-    const int bb = at.chain / groups, ch = at.chain % groups * kGroup + 2 * lane;
+    const int bb = at.bb, ch = at.cg * kGroup + 2 * lane;
     const Early early = look(p, at, warp, lane);
     float2 h = *reinterpret_cast<const float2*>(p.kept + ((size_t)bb * p.tiles + tile) * p.HD + ch);
-    int later = tickets.total;
-    if (tickets.more) {
-      if (!tickets.drawn) later = next + (int)gridDim.x;
-      else if (threadIdx.x == 0) later = tickets.draw(p);
-    }
+    if (threadIdx.x == 0) tickets.ask(p, false);
     float2 na[kRows], nd[kRows];
-    const bool on = tickets.is(next);
+    const bool on = next.k >= 0;
     if (begin) fetched<0>();
     if (on) fold(next, na, nd, coming);
     fetched<0>();
@@ -589,12 +606,12 @@ __global__ void __launch_bounds__(256, 2) k_recur_bwd(const Args p) {
       m = after({a[r], mul2(w, v)}, m);
     }
     __syncthreads();
-    if (warp == 1 && on) publish_map(p, tickets.place(p, next), coming, lane);
-    if (threadIdx.x == 0) joint.ticket[0] = later;
+    if (warp == 1 && on) publish_map(p, next, coming, lane);
+    if (threadIdx.x == 0) joint.place[0] = tickets.place(p);
     fmap[warp][lane] = flat(m);
     join(p, at, map, joint, p.dhf, early, warp, lane);
     __syncthreads();
-    if (tickets.drawn) later = joint.ticket[0];
+    const Place later = told(joint.place[0]);
     prefetch(later);
     h = walk(fmap, warp, lane, h);
     float2 c = walk(map, back, lane, entering(joint, lane));
