@@ -57,23 +57,33 @@ template <> struct Vec<__nv_bfloat16> {
 
 constexpr int kUnroll = 4;   // 16-byte pieces a thread holds at once
 
-// Codes of the kUnroll pieces of a thread, one word per 4 values, and in `scale`
+// Codes of the kUnroll pieces of a thread, one word per 4 values, and as the value
 // the scale of piece (lane & 3): a group's lanes share its division (every lane
 // dividing for every piece cost a third of the instructions).  Whole warps call.
-template <int E>
-__device__ __forceinline__ float encode(const float (&x)[kUnroll][E], unsigned (&word)[kUnroll][E / 4]) {
+// clip > 0: through the sanitiser, looked at only where a maximum asks for it.
+template <typename T>
+__device__ __forceinline__ float encode(float (&x)[kUnroll][Vec<T>::E],
+                                        unsigned (&word)[kUnroll][Vec<T>::E / 4], float clip = 0.f) {
+  constexpr int E = Vec<T>::E;
   float mine = 0.f;
 #pragma unroll
   for (int u = 0; u < kUnroll; ++u) {
-    float top = fabsf(x[u][0]);
+    auto largest = [&] {
+      float t = 0.f;
 #pragma unroll
-    for (int i = 1; i < E; ++i) top = max_abs(top, x[u][i]);
+      for (int i = 0; i < E; i += 2) t = max_abs3(t, x[u][i], x[u][i + 1]);
 #pragma unroll
-    for (int o = 1; o < kGroup / E; o <<= 1)
-      top = max_abs(top, __shfl_xor_sync(0xffffffffu, top, o));
-    const float inv = group_inv(top);
+      for (int o = 1; o < kGroup / E; o <<= 1) t = max_abs(t, __shfl_xor_sync(0xffffffffu, t, o));
+      return t;
+    };
+    float top = largest();
+    if (clip > 0.f && __any_sync(0xffffffffu, !(top <= clip))) {
+#pragma unroll
+      for (int i = 0; i < E; ++i) x[u][i] = san(x[u][i], clip);
+      top = largest();
+    }
     unsigned c[E];
-    int8_codes<E>(x[u], inv, top, c);
+    int8_codes<T, E>(x[u], top, c);
 #pragma unroll
     for (int i = 0; i < E; i += 4) word[u][i / 4] = pack4(c[i], c[i + 1], c[i + 2], c[i + 3]);
     if ((threadIdx.x & 3) == u) mine = top;
@@ -128,7 +138,7 @@ __global__ void __launch_bounds__(256) k_pack(Tensors a, size_t n) {
     if (i < n) Vec<T>::load(v[u], x + i);
   }
   unsigned w[kUnroll][E / 4];
-  const float scale = encode<E>(v, w);
+  const float scale = encode<T>(v, w);
 #pragma unroll
   for (int u = 0; u < kUnroll; ++u) {
     const size_t i = base + (size_t)u * 256 * E;
@@ -187,12 +197,8 @@ k_state_write(const float* __restrict__ h, int8_t* __restrict__ codes, float* __
   if (__syncthreads_or(later) || slot < 0 || slot >= S) return;
   int8_t* c = codes + (size_t)slot * n;
   float* s = scales + (size_t)slot * (n / kGroup);
-#pragma unroll
-  for (int u = 0; u < kUnroll; ++u)
-#pragma unroll
-    for (int k = 0; k < E; ++k) v[u][k] = san(v[u][k], clip);
   unsigned w[kUnroll][1];
-  const float scale = encode<E>(v, w);
+  const float scale = encode<float>(v, w, clip);
 #pragma unroll
   for (int u = 0; u < kUnroll; ++u) {
     const size_t i = base + (size_t)u * 256 * E;

@@ -90,50 +90,59 @@ static __device__ __noinline__ float int8_border(float x, float y, float top) {
   return copysignf(lo + (up ? 1.f : 0.f), x);
 }
 // The codes of N (even) values of one group, each in the low byte of a word.
-// kCodeBias added to y = x * inv, |y| <= 127.01, rounds it to a whole number in the
-// low bits (the conversion and rounding instructions run at an eighth of the
-// rate).  y is off by at most 127 * 2^-22.5 = 2.2e-5, so only a y within 1e-4 of
-// a half can round the wrong way: one value in 5000 is decided in float64.
+// kCodeBias added to y, |y| <= 127.01, rounds it to a whole number in the low bits
+// (the conversion and rounding instructions run at an eighth of the rate).
+//
+// float32: y = x * inv is off by at most 127 * 2^-22.5 = 2.2e-5, so only a y within
+// 3e-5 of a half can round the wrong way; one value in 17000 is decided in float64.
 template <int N>
-__device__ __forceinline__ float int8_near(const float (&x)[N], float inv, unsigned (&code)[N]) {
+__device__ __forceinline__ void int8_codes_f32(const float (&x)[N], float top, unsigned (&code)[N]) {
+  const float inv = group_inv(top);
   float far = 0.f;   // the largest distance of a y from its code
 #pragma unroll
   for (int i = 0; i < N; i += 2) {
     const float2 v = make_float2(x[i], x[i + 1]), t = fma2(v, both(inv), both(kCodeBias));
     const float2 r = fma2(v, both(inv), fma2(t, both(-1.f), both(kCodeBias)));
-    far = fmaxf(far, fmaxf(fabsf(r.x), fabsf(r.y)));
+    far = max_abs3(far, r.x, r.y);
     code[i] = __float_as_uint(t.x);
     code[i + 1] = __float_as_uint(t.y);
   }
-  return far;
-}
-template <int N>
-__device__ __forceinline__ void int8_decide(const float (&x)[N], float inv, float top, unsigned (&code)[N]) {
+  if (far > 0.49997f) {
 #pragma unroll
-  for (int i = 0; i < N; ++i) {
-    const float y = x[i] * inv, r = __uint_as_float(code[i]) - kCodeBias;
-    if (fabsf(y - r) > 0.4998f)
-      code[i] = __float_as_uint(int8_border(x[i], y, top) + kCodeBias);
+    for (int i = 0; i < N; ++i) {
+      const float y = x[i] * inv, r = __uint_as_float(code[i]) - kCodeBias;
+      if (fabsf(y - r) > 0.4999f)
+        code[i] = __float_as_uint(int8_border(x[i], y, top) + kCodeBias);
+    }
   }
 }
+// bf16: exact ties are common (8-bit mantissas: one value in 500), but 127 x / top
+// is either a half or at least 2^-16 away from it, and one correction makes the
+// quotient exact where it is a half: with q = x * inv the remainder 127 x - q top
+// has 10 bits and is exact, and q + remainder / top rounds to the quotient.
 template <int N>
-__device__ __forceinline__ void int8_codes(const float (&x)[N], float inv, float top,
-                                           unsigned (&code)[N]) {
-  if (int8_near(x, inv, code) > 0.4999f) int8_decide(x, inv, top, code);
+__device__ __forceinline__ void int8_codes_bf16(const float (&x)[N], float top, unsigned (&code)[N]) {
+  const float f = top > 0x1p100f ? 0x1p-100f : 1.f;   // 127 x stays finite
+  const float t1 = top * f, c1 = 127.f * f;
+  float rc;
+  asm("rcp.approx.f32 %0, %1;" : "=f"(rc) : "f"(fmaxf(t1, kInt8Tiny)));
+  const float inv = c1 * rc;
+#pragma unroll
+  for (int i = 0; i < N; i += 2) {
+    const float2 v = make_float2(x[i], x[i + 1]), q = mul2(v, both(inv));
+    const float2 r = fma2(q, both(-t1), mul2(v, both(c1)));
+    const float2 t = add2(fma2(r, both(rc), q), both(kCodeBias));
+    code[i] = __float_as_uint(t.x);
+    code[i + 1] = __float_as_uint(t.y);
+  }
+}
+template <typename T, int N>
+__device__ __forceinline__ void int8_codes(const float (&x)[N], float top, unsigned (&code)[N]) {
+  if constexpr (sizeof(T) == 4) int8_codes_f32(x, top, code);
+  else int8_codes_bf16(x, top, code);
 }
 __device__ __forceinline__ unsigned pack4(unsigned a, unsigned b, unsigned c, unsigned d) {
   return __byte_perm(__byte_perm(a, b, 0x0040), __byte_perm(c, d, 0x0040), 0x5410);
-}
-// Two values each of two groups: the four codes as bytes.
-__device__ __forceinline__ unsigned int8_codes2x2(float2 v, float2 w, float tv, float tw) {
-  const float x[2] = {v.x, v.y}, y[2] = {w.x, w.y}, iv = group_inv(tv), iw = group_inv(tw);
-  unsigned c[2], d[2];
-  const float far = int8_near(x, iv, c);
-  if (fmaxf(far, int8_near(y, iw, d)) > 0.4999f) {
-    int8_decide(x, iv, tv, c);
-    int8_decide(y, iw, tw, d);
-  }
-  return pack4(c[0], c[1], d[0], d[1]);
 }
 // Byte I of four codes as a float: the code moved to 0..255 becomes the low
 // byte of 2^23 + code, and one exact subtraction takes both offsets off (the

@@ -227,9 +227,11 @@ struct Tickets {
 };
 __device__ __forceinline__ Place told(const int4& z) { return {z.x, z.y, z.z, z.w}; }
 
-// How a tile of a chain gets the state that enters it (map: the maps of its warps
-// in the order of the scan).
+// How a tile of a chain gets the state that enters it.
+using Maps = float4[kWarps][32];   // of the warps, in the order of the scan
 struct Joint {
+  Maps maps;                  // of the warps of one tile
+  Maps upto[2];               // [w]: warps 0 .. w, of the present and the next tile
   float4 pairs[kWarps][32];   // the mates 2 w and 2 w + 1 before it in its group
   float2 enter[32];           // the state that enters the group
   int4 place[2];
@@ -240,29 +242,42 @@ __device__ __forceinline__ ulonglong2* map_of(const Args& p, Place at, int k, in
 __device__ __forceinline__ ulonglong2* enter_of(const Args& p, Place at, int group, int lane) {
   return p.s.enter + ((size_t)group * p.chains + at.chain) * 32 + lane;
 }
-// One warp publishes a tile's map, where another tile will look at it.
-__device__ __forceinline__ void publish_map(const Args& p, Place at, const float4 (*map)[32], int lane) {
-  if (at.k + 1 == p.tiles || at.k % kGroupTiles == kGroupTiles - 1) return;
-  Map m = unflat(map[0][lane]);
+// One warp: maps -> the maps of warps 0 .. w, the whole tile's last.
+__device__ __forceinline__ Map prefixes(const Maps& maps, Maps& upto, int lane) {
+  Map m[kWarps];   // all loads before the first store, which they could alias for the compiler
 #pragma unroll
-  for (int j = 1; j < kWarps; ++j) m = after(unflat(map[j][lane]), m);
-  publish(map_of(p, at, at.k, lane), m);
+  for (int j = 0; j < kWarps; ++j) m[j] = unflat(maps[j][lane]);
+#pragma unroll
+  for (int j = 1; j < kWarps; ++j) m[j] = after(m[j], m[j - 1]);
+#pragma unroll
+  for (int j = 0; j < kWarps; ++j) upto[j][lane] = flat(m[j]);
+  return m[kWarps - 1];
 }
-// What a warp needs of others, looked at long before it is needed.
-struct Early { ulonglong2 even, odd, enter; };
+__device__ __forceinline__ float2 past(const Maps& upto, int warps, int lane, float2 h) {
+  return warps ? apply(unflat(upto[warps - 1][lane]), h) : h;
+}
+// The same warp publishes the tile's map, where another tile will look at it.
+__device__ __forceinline__ void publish_map(const Args& p, Place at, Map m, int lane) {
+  if (at.k + 1 < p.tiles && at.k % kGroupTiles != kGroupTiles - 1)
+    publish(map_of(p, at, at.k, lane), m);
+}
+// What a warp needs of others, looked at long before it is needed: two mates, or
+// for the last warp, whose second mate a group never has, the group's entering
+// state.
+struct Early { ulonglong2 even, odd; };
 __device__ __forceinline__ Early look(const Args& p, Place at, int warp, int lane) {
   const int mate = at.k % kGroupTiles, group = at.k / kGroupTiles;
   Early e{};
   if (2 * warp < mate) e.even = peek(map_of(p, at, at.k - mate + 2 * warp, lane));
   if (2 * warp + 1 < mate) e.odd = peek(map_of(p, at, at.k - mate + 2 * warp + 1, lane));
-  if (warp == 0 && group) e.enter = peek(enter_of(p, at, group, lane));
+  if (warp == kWarps - 1 && group) e.odd = peek(enter_of(p, at, group, lane));
   return e;
 }
 __device__ __forceinline__ Map have(ulonglong2 early, const ulonglong2* p, int* status) {
   return __all_sync(0xffffffffu, there(early)) ? unword(early) : await(p, status);
 }
 // All warps, between two synchronisations of the CTA; fills `joint`.
-__device__ __forceinline__ void join(const Args& p, Place at, const float4 (*map)[32], Joint& joint,
+__device__ __forceinline__ void join(const Args& p, Place at, const Maps& upto, Joint& joint,
                                      const float* first, const Early& e, int warp, int lane) {
   const int mate = at.k % kGroupTiles, group = at.k / kGroupTiles, k0 = at.k - mate + 2 * warp;
   const bool hands_on = mate == kGroupTiles - 1 && at.k + 1 < p.tiles;
@@ -274,17 +289,17 @@ __device__ __forceinline__ void join(const Args& p, Place at, const float4 (*map
     // the step from group to group is the dependent one: everything else of it
     // is joined before the wait
     __syncthreads();
-    if (warp == 0) {
+    if (warp == kWarps - 1) {
+      m = unflat(joint.pairs[0][lane]);
 #pragma unroll
       for (int i = 1; i < kWarps; ++i) m = after(unflat(joint.pairs[i][lane]), m);
-#pragma unroll
-      for (int j = 0; j < kWarps; ++j) m = after(unflat(map[j][lane]), m);
+      m = after(unflat(upto[kWarps - 1][lane]), m);
     }
   }
-  if (warp == 0) {
+  if (warp == kWarps - 1) {
     float2 h = both(0.f);
     if (group)
-      h = have(e.enter, enter_of(p, at, group, lane), p.s.status).b;
+      h = have(e.odd, enter_of(p, at, group, lane), p.s.status).b;
     else if (first)
       h = *reinterpret_cast<const float2*>(first + (size_t)at.chain * kGroup + 2 * lane);
     if (hands_on) publish(enter_of(p, at, group + 1, lane), {both(0.f), apply(m, h)});
@@ -297,34 +312,54 @@ __device__ __forceinline__ float2 entering(const Joint& joint, int lane) {
   for (int i = 0; i < kWarps; ++i) h = apply(unflat(joint.pairs[i][lane]), h);
   return h;
 }
-// Through the maps of a tile's warps before `count`.
-__device__ __forceinline__ float2 walk(const float4 (*map)[32], int count, int lane, float2 h) {
+// The int8 form of a warp's 8 rows (groups) of one tensor: 4 lanes take a row, 16
+// values each, so a group's maximum takes two shuffles, every lane's division is
+// a group's, and its codes leave as one 16-byte store.  (Lanes of two channels,
+// as the recurrence has them, took 37 instructions a row instead of 10.)
+template <typename T>
+__device__ __forceinline__ void put_int8(const T (*x)[kGroup], int8_t* codes, float* scales,
+                                         size_t stride, int groups, int rows, int lane) {
+  constexpr int E = 16 / sizeof(T), N = 16 / E;   // values of a 16-byte piece; pieces of a lane
+  const int r = lane >> 2, q = lane & 3;
+  float v[16], top = 0.f;
 #pragma unroll
-  for (int j = 0; j < kWarps - 1; ++j) {
-    const float2 x = apply(unflat(map[j][lane]), h);
-    h = j < count ? x : h;
-  }
-  return h;
-}
-
-// The int8 forms of a warp's 16 groups (8 rows of two tensors): codes are
-// stored here, lane 2 r + j keeps the scale of tensor j's row r (one division a
-// lane instead of one a group).
-__device__ __forceinline__ float put_int8(const float2 (&v)[kRows], const float2 (&w)[kRows],
-                                          int8_t* v8, int8_t* w8, size_t stride, int rows, int lane) {
-  float mine = 0.f;
+  for (int i = 0; i < N; ++i) {
+    // the quarter's pieces in an order of its own: fewer lanes on one bank
+    const int piece = (i + q) % N;
+    const uint4 u = *reinterpret_cast<const uint4*>(&x[r][q * 16 + piece * E]);
+    const unsigned w[4] = {u.x, u.y, u.z, u.w};
 #pragma unroll
-  for (int r = 0; r < kRows; ++r) {
-    const float tv = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(max_abs(v[r].x, v[r].y))));
-    const float tw = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(max_abs(w[r].x, w[r].y))));
-    const unsigned c = int8_codes2x2(v[r], w[r], tv, tw);
-    if (r < rows) {
-      *reinterpret_cast<unsigned short*>(v8 + r * stride) = (unsigned short)c;
-      *reinterpret_cast<unsigned short*>(w8 + r * stride) = (unsigned short)(c >> 16);
+    for (int k = 0; k < 4; ++k) {
+      if constexpr (E == 4) v[i * 4 + k] = __uint_as_float(w[k]);
+      else {
+        v[i * 8 + 2 * k] = __uint_as_float(w[k] << 16);
+        v[i * 8 + 2 * k + 1] = __uint_as_float(w[k] & 0xffff0000u);
+      }
     }
-    mine = lane == 2 * r ? tv : lane == 2 * r + 1 ? tw : mine;
   }
-  return group_scale(mine);
+#pragma unroll
+  for (int i = 0; i < 16; i += 2) top = max_abs3(top, v[i], v[i + 1]);
+  top = max_abs(top, __shfl_xor_sync(0xffffffffu, top, 1));
+  top = max_abs(top, __shfl_xor_sync(0xffffffffu, top, 2));
+  unsigned c[16];
+  int8_codes<T, 16>(v, top, c);
+  unsigned word[4], out[4];   // word i: in the order of the loads
+#pragma unroll
+  for (int i = 0; i < 4; ++i) word[i] = pack4(c[4 * i], c[4 * i + 1], c[4 * i + 2], c[4 * i + 3]);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {   // turned back by q pieces of 4 / N words
+    if constexpr (N == 4) {
+      const unsigned one = q & 1 ? word[(i + 3) & 3] : word[i];
+      const unsigned two = q & 1 ? word[(i + 1) & 3] : word[(i + 2) & 3];
+      out[i] = q & 2 ? two : one;
+    } else {
+      out[i] = q & 1 ? word[i ^ 2] : word[i];
+    }
+  }
+  if (r < rows) {
+    *reinterpret_cast<uint4*>(codes + r * stride + q * 16) = make_uint4(out[0], out[1], out[2], out[3]);
+    if (q == 0) scales[(size_t)r * groups] = group_scale(top);
+  }
 }
 
 // Where a tile lies for a warp: rows of it (8 and more: all eight), first element.
@@ -334,17 +369,43 @@ __device__ __forceinline__ Rows rows_of(const Args& p, Place at, int tile, int w
   return {p.T - t0, ((size_t)at.bb * p.T + t0) * p.HD + at.cg * kGroup};
 }
 
+// The first two tiles of a CTA: the first is folded and published, the second on
+// its way.  False where there is none.
+template <typename Prefetch, typename Fold>
+__device__ __forceinline__ bool begin(const Args& p, Tickets& tickets, Joint& joint, Place& now,
+                                      Place& next, Prefetch prefetch, Fold fold, int warp, int lane) {
+  if (threadIdx.x == 0) {
+    tickets.ask(p, true);
+    joint.place[0] = tickets.place(p);
+  }
+  __syncthreads();
+  now = told(joint.place[0]);
+  if (now.k < 0) return false;
+  prefetch(now);
+  fold(now);
+  // the second ticket once the first tile's bytes are there, when other CTAs have
+  // theirs: one that drew two at once would leave another without any
+  if (threadIdx.x == 0) {
+    tickets.ask(p, false);
+    joint.place[1] = tickets.place(p);
+  }
+  __syncthreads();
+  next = told(joint.place[1]);
+  prefetch(next);
+  if (warp == 1) publish_map(p, now, prefixes(joint.maps, joint.upto[0], lane), lane);
+  __syncthreads();
+  return true;
+}
+
 // Shared memory of a warp: its 8 rows of the tile that comes next.
 template <typename T> struct FwdStage { T g[kRows][kGroup], v[kRows][kGroup], w[kRows][kGroup]; };
 
 template <typename T, bool SAVE8, bool RAW>
 __global__ void __launch_bounds__(256, 2) k_recur_fwd(const Args p) {
   extern __shared__ __align__(16) unsigned char raw_stage[];
-  __shared__ float4 maps[3][kWarps][32];   // of the present tile, the next and the one before
   __shared__ Joint joint;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   FwdStage<T>& st = reinterpret_cast<FwdStage<T>*>(raw_stage)[warp];
-  const int groups = p.HD / kGroup;
   Tickets tickets(p);
   auto prefetch = [&](Place at) {
     if (at.k >= 0) {
@@ -355,38 +416,21 @@ __global__ void __launch_bounds__(256, 2) k_recur_fwd(const Args p) {
     }
     fetch_end();
   };
-  // the rows of tile t as maps (a, x), and the map of the warp
-  auto fold = [&](Place at, float2 (&a)[kRows], float2 (&x)[kRows], float4 (*map)[32]) {
+  // the rows of a tile as maps (a, x), and the map of the warp
+  auto fold = [&](Place at, float2 (&a)[kRows], float2 (&x)[kRows]) {
     const Rows z = rows_of(p, at, at.k, warp);
-    typename Raw<T>::type rg[kRows], rv[kRows], rw[kRows];
     fetched<0>();
+    if constexpr (SAVE8) {
+      put_int8(st.v, p.v8 + z.i, p.vs + z.i / kGroup, p.HD, p.HD / kGroup, z.rows, lane);
+      put_int8(st.w, p.w8 + z.i, p.ws + z.i / kGroup, p.HD, p.HD / kGroup, z.rows, lane);
+    }
 #pragma unroll
     for (int r = 0; r < kRows; ++r) {
-      rg[r] = ldraw(&st.g[r][2 * lane]);
-      rv[r] = ldraw(&st.v[r][2 * lane]);
-      rw[r] = ldraw(&st.w[r][2 * lane]);
+      a[r] = decay2<RAW>(value2(ldraw(&st.g[r][2 * lane])));
+      x[r] = mul2(gate2<RAW>(value2(ldraw(&st.w[r][2 * lane]))), value2(ldraw(&st.v[r][2 * lane])));
     }
     __syncwarp();
-    if constexpr (SAVE8) {
-      if (z.rows > 0) {
-        float2 v[kRows], w[kRows];
-#pragma unroll
-        for (int r = 0; r < kRows; ++r) {
-          v[r] = value2(rv[r]);
-          w[r] = value2(rw[r]);
-        }
-        const float scale = put_int8(v, w, p.v8 + z.i + 2 * lane, p.w8 + z.i + 2 * lane, p.HD,
-                                     z.rows, lane);
-        if (lane < 2 * min(z.rows, kRows))
-          (lane & 1 ? p.ws : p.vs)[z.i / kGroup + (size_t)(lane >> 1) * groups] = scale;
-      }
-    }
-#pragma unroll
-    for (int r = 0; r < kRows; ++r) {
-      a[r] = decay2<RAW>(value2(rg[r]));
-      x[r] = mul2(gate2<RAW>(value2(rw[r])), value2(rv[r]));
-    }
-    if (z.rows < kRows) {
+    if (z.rows < kRows) {   // rows behind the end keep the state
 #pragma unroll
       for (int r = 0; r < kRows; ++r)
         if (r >= z.rows) a[r] = both(1.f), x[r] = both(0.f);
@@ -394,67 +438,46 @@ __global__ void __launch_bounds__(256, 2) k_recur_fwd(const Args p) {
     Map m = {a[0], x[0]};
 #pragma unroll
     for (int r = 1; r < kRows; ++r) m = after({a[r], x[r]}, m);
-    map[warp][lane] = flat(m);
+    joint.maps[warp][lane] = flat(m);
   };
 
-  if (threadIdx.x == 0) {
-    tickets.ask(p, true);
-    joint.place[0] = tickets.place(p);
-  }
-  __syncthreads();
-  Place now = told(joint.place[0]);
-  if (now.k < 0) return;
-  prefetch(now);
-  float2 a[kRows], x[kRows];
-  fold(now, a, x, maps[0]);
-  // the second ticket once the first tile's bytes are there, when other CTAs have
-  // theirs: one that drew two at once would leave another without any
-  if (threadIdx.x == 0) {
-    tickets.ask(p, false);
-    joint.place[1] = tickets.place(p);
-  }
-  __syncthreads();
-  Place next = told(joint.place[1]);
-  prefetch(next);
-  if (warp == 1) publish_map(p, now, maps[0], lane);
-  for (int turn = 0; now.k >= 0; turn = turn == 2 ? 0 : turn + 1) {
-    const float4 (*map)[32] = maps[turn];
-    float4 (*coming)[32] = maps[turn == 2 ? 0 : turn + 1];
-    const Place at = now;
-    const Early early = look(p, at, warp, lane);
+  Place now, next;
+  float2 a[2][kRows], x[2][kRows];
+  if (!begin(p, tickets, joint, now, next, prefetch, [&](Place at) { fold(at, a[0], x[0]); }, warp, lane))
+    return;
+  // One tile: `me` of the two register sets holds it, the other takes the next.
+  auto turn = [&](auto me) {
+    constexpr int N = decltype(me)::value, M = N ^ 1;
+    const Early early = look(p, now, warp, lane);
     if (threadIdx.x == 0) tickets.ask(p, false);
-    float2 na[kRows], nx[kRows];
     const bool on = next.k >= 0;
-    if (on) fold(next, na, nx, coming);
+    if (on) fold(next, a[M], x[M]);
     __syncthreads();
-    if (warp == 1 && on) publish_map(p, next, coming, lane);
+    if (warp == 1 && on) publish_map(p, next, prefixes(joint.maps, joint.upto[M], lane), lane);
     if (threadIdx.x == 0) joint.place[0] = tickets.place(p);
-    join(p, at, map, joint, p.h0, early, warp, lane);
+    join(p, now, joint.upto[N], joint, p.h0, early, warp, lane);
     __syncthreads();
     const Place later = told(joint.place[0]);
     prefetch(later);
-    const Rows z = rows_of(p, at, at.k, warp);
-    const int bb = at.bb, ch = at.cg * kGroup + 2 * lane;
+    const Rows z = rows_of(p, now, now.k, warp);
+    const int ch = now.cg * kGroup + 2 * lane;
     float2 h = entering(joint, lane);
     if (warp == 0 && p.kept)
-      *reinterpret_cast<float2*>(p.kept + ((size_t)bb * p.tiles + at.k) * p.HD + ch) = h;
-    h = walk(map, warp, lane, h);
+      *reinterpret_cast<float2*>(p.kept + ((size_t)now.bb * p.tiles + now.k) * p.HD + ch) = h;
+    h = past(joint.upto[N], warp, lane, h);
     float* o = p.o + z.i + 2 * lane;
 #pragma unroll
     for (int r = 0; r < kRows; ++r) {
-      h = apply({a[r], x[r]}, h);
+      h = apply({a[N][r], x[N][r]}, h);
       if (r < z.rows) st2(o + (size_t)r * p.HD, h);
     }
-    // rows behind the end keep the state
     if (z.rows > 0 && z.rows <= kRows)
-      *reinterpret_cast<float2*>(p.hf + (size_t)bb * p.HD + ch) = h;
-#pragma unroll
-    for (int r = 0; r < kRows; ++r) {
-      a[r] = na[r];
-      x[r] = nx[r];
-    }
+      *reinterpret_cast<float2*>(p.hf + (size_t)now.bb * p.HD + ch) = h;
     now = next;
     next = later;
+    return now.k >= 0;
+  };
+  while (turn(std::integral_constant<int, 0>{}) && turn(std::integral_constant<int, 1>{})) {
   }
 }
 
@@ -495,18 +518,17 @@ template <typename T, typename V> struct BwdStage {
 };
 
 // Tiles in the order of the reverse scan: k = 0 is the last one in time, and the
-// maps of its warps are kept from the last warp to the first.
+// maps of its warps stand from the last warp to the first.
 template <typename T, bool FROM8, bool RAW>
 __global__ void __launch_bounds__(256, 2) k_recur_bwd(const Args p) {
   using V = typename std::conditional<FROM8, int8_t, T>::type;
   extern __shared__ __align__(16) unsigned char raw_stage[];
-  __shared__ float4 maps[3][kWarps][32], fmap[kWarps][32];
   __shared__ Joint joint;
+  __shared__ Maps fmaps, fupto;   // of the present tile's states, in the order of time
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, back = kWarps - 1 - warp;
   BwdStage<T, V>& st = reinterpret_cast<BwdStage<T, V>*>(raw_stage)[warp];
   const V* pv = FROM8 ? reinterpret_cast<const V*>(p.v8) : static_cast<const V*>(p.v);
   const V* pw = FROM8 ? reinterpret_cast<const V*>(p.w8) : static_cast<const V*>(p.w);
-  const int groups = p.HD / kGroup;
   Tickets tickets(p);
   auto prefetch = [&](Place at) {
     if (at.k >= 0) {
@@ -522,34 +544,34 @@ __global__ void __launch_bounds__(256, 2) k_recur_bwd(const Args p) {
       fetch(&st.v[0][0], pv + z.i, p.HD, z.rows, lane);
       fetch(&st.w[0][0], pw + z.i, p.HD, z.rows, lane);
       if (FROM8 && lane < 2 * min(z.rows, kRows))
-        fetch4(&st.scale[lane], (lane & 1 ? p.ws : p.vs) + z.i / kGroup + (size_t)(lane >> 1) * groups);
+        fetch4(&st.scale[lane], (lane & 1 ? p.ws : p.vs) + z.i / kGroup +
+                                    (size_t)(lane >> 1) * (p.HD / kGroup));
     }
     fetch_end();
   };
-  // decays and cotangents of tile t, and the warp's map of the reverse scan
-  auto fold = [&](Place at, float2 (&a)[kRows], float2 (&d)[kRows], float4 (*map)[32]) {
-    const Rows z = rows_of(p, at, p.tiles - 1 - at.k, warp);
+  // decays and cotangents of a tile, and the warp's map of the reverse scan
+  auto fold = [&](Place at, float2 (&a)[kRows], float2 (&d)[kRows]) {
+    const int rows = p.T - (p.tiles - 1 - at.k) * kTile - warp * kRows;
     fetched<1>();
 #pragma unroll
     for (int r = 0; r < kRows; ++r) {
-      a[r] = value2(ldraw(&st.g[r][2 * lane]));
+      a[r] = decay2<RAW>(value2(ldraw(&st.g[r][2 * lane])));
       d[r] = ldraw(&st.d[r][2 * lane]);
     }
     __syncwarp();
-#pragma unroll
-    for (int r = 0; r < kRows; ++r) a[r] = decay2<RAW>(a[r]);
-    if (z.rows < kRows) {
+    if (rows < kRows) {   // rows behind the end hand the cotangent on
 #pragma unroll
       for (int r = 0; r < kRows; ++r)
-        if (r >= z.rows) a[r] = both(1.f), d[r] = both(0.f);
+        if (r >= rows) a[r] = both(1.f), d[r] = both(0.f);
     }
     Map m = identity();
 #pragma unroll
     for (int r = kRows - 1; r >= 0; --r) m = {mul2(a[r], m.a), mul2(a[r], add2(d[r], m.b))};
-    map[back][lane] = flat(m);
+    joint.maps[back][lane] = flat(m);
   };
-  // v and w of row r of the present tile
-  auto vw = [&](int r, int rows, float2& v, float2& w) {
+  // v and w of row r of the present tile; behind the end anything: only states
+  // that nothing reads come of it
+  auto vw = [&](int r, float2& v, float2& w) {
     v = value2(ldraw(&st.v[r][2 * lane]));
     w = value2(ldraw(&st.w[r][2 * lane]));
     if constexpr (FROM8) {
@@ -557,81 +579,64 @@ __global__ void __launch_bounds__(256, 2) k_recur_bwd(const Args p) {
       w = mul2(w, both(st.scale[2 * r + 1]));
     }
     w = gate2<RAW>(w);
-    if (r >= rows) v = w = both(0.f);
   };
 
-  if (threadIdx.x == 0) {
-    tickets.ask(p, true);
-    joint.place[0] = tickets.place(p);
-  }
-  __syncthreads();
-  Place now = told(joint.place[0]);
-  if (now.k < 0) return;
-  prefetch(now);
-  prefetch_vw(now);
-  float2 a[kRows], d[kRows];
-  fold(now, a, d, maps[0]);
-  // the second ticket once the first tile's bytes are there, when other CTAs have
-  // theirs: one that drew two at once would leave another without any
-  if (threadIdx.x == 0) {
-    tickets.ask(p, false);
-    joint.place[1] = tickets.place(p);
-  }
-  __syncthreads();
-  Place next = told(joint.place[1]);
-  prefetch(next);
-  if (warp == 1) publish_map(p, now, maps[0], lane);
-  // in flight here and at the end of each turn: v, w of `now` and g, dout of
-  // `next`, the one that is needed first first
-  for (int turn = 0, begin = 1; now.k >= 0; turn = turn == 2 ? 0 : turn + 1, begin = 0) {
-    const float4 (*map)[32] = maps[turn];
-    float4 (*coming)[32] = maps[turn == 2 ? 0 : turn + 1];
-    const Place at = now;
-    const int tile = p.tiles - 1 - at.k;
-    const Rows z = rows_of(p, at, tile, warp);
-    const int bb = at.bb, ch = at.cg * kGroup + 2 * lane;
-    const Early early = look(p, at, warp, lane);
-    float2 h = *reinterpret_cast<const float2*>(p.kept + ((size_t)bb * p.tiles + tile) * p.HD + ch);
+  Place now, next;
+  float2 a[2][kRows], d[2][kRows];
+  if (!begin(p, tickets, joint, now, next, prefetch, [&](Place at) {
+        prefetch_vw(at);
+        fold(at, a[0], d[0]);
+      }, warp, lane))
+    return;
+  // in flight at the end of each turn: g, dout of the next tile, then v, w of the
+  // present one; here, once, the other way round
+  fetched<0>();
+  int side = 0;
+  auto turn = [&](auto me) {
+    constexpr int N = decltype(me)::value, M = N ^ 1;
+    const int tile = p.tiles - 1 - now.k, ch = now.cg * kGroup + 2 * lane;
+    const Rows z = rows_of(p, now, tile, warp);
+    const Early early = look(p, now, warp, lane);
+    float2 h = *reinterpret_cast<const float2*>(p.kept + ((size_t)now.bb * p.tiles + tile) * p.HD + ch);
     if (threadIdx.x == 0) tickets.ask(p, false);
-    float2 na[kRows], nd[kRows];
     const bool on = next.k >= 0;
-    if (begin) fetched<0>();
-    if (on) fold(next, na, nd, coming);
+    if (on) fold(next, a[M], d[M]);
     fetched<0>();
+    float2 x[kRows];   // w v, then the state before each row
     Map m = identity();
 #pragma unroll
     for (int r = 0; r < kRows; ++r) {
       float2 v, w;
-      vw(r, z.rows, v, w);
-      m = after({a[r], mul2(w, v)}, m);
+      vw(r, v, w);
+      x[r] = mul2(w, v);
+      m = after({a[N][r], x[r]}, m);
     }
+    fmaps[warp][lane] = flat(m);
     __syncthreads();
-    if (warp == 1 && on) publish_map(p, next, coming, lane);
+    if (warp == 1 && on) publish_map(p, next, prefixes(joint.maps, joint.upto[side ^ 1], lane), lane);
+    if (warp == 2) prefixes(fmaps, fupto, lane);
     if (threadIdx.x == 0) joint.place[0] = tickets.place(p);
-    fmap[warp][lane] = flat(m);
-    join(p, at, map, joint, p.dhf, early, warp, lane);
+    join(p, now, joint.upto[side], joint, p.dhf, early, warp, lane);
     __syncthreads();
     const Place later = told(joint.place[0]);
     prefetch(later);
-    h = walk(fmap, warp, lane, h);
-    float2 c = walk(map, back, lane, entering(joint, lane));
-    float2 before[kRows];
+    h = past(fupto, warp, lane, h);
+    float2 c = past(joint.upto[side], back, lane, entering(joint, lane));
 #pragma unroll
     for (int r = 0; r < kRows; ++r) {
-      float2 v, w;
-      vw(r, z.rows, v, w);
-      before[r] = h;
-      h = apply({a[r], mul2(w, v)}, h);
+      const float2 after_r = apply({a[N][r], x[r]}, h);
+      x[r] = h;
+      h = after_r;
     }
 #pragma unroll
     for (int r = kRows - 1; r >= 0; --r) {
-      const float2 dh = add2(d[r], c);
-      c = mul2(a[r], dh);
+      const float2 dh = add2(d[N][r], c);
+      c = mul2(a[N][r], dh);
       if (r < z.rows) {
         const size_t i = z.i + 2 * lane + (size_t)r * p.HD;
         float2 v, w;
-        vw(r, kRows, v, w);
-        float2 dw = mul2(v, dh), dg = mul2(before[r], c);
+        vw(r, v, w);
+        float2 dw = mul2(v, dh), dg = mul2(x[r], c);
         if constexpr (RAW) {
           // d sigmoid(x) = w (1 - w); dg/dx = -sigmoid(x)
           dw = make_float2(dw.x * (w.x * (1.f - w.x)), dw.y * (w.y * (1.f - w.y)));
@@ -643,16 +648,22 @@ __global__ void __launch_bounds__(256, 2) k_recur_bwd(const Args p) {
         st2(static_cast<T*>(p.dg) + i, dg);
       }
     }
-    if (tile == 0 && warp == 0) *reinterpret_cast<float2*>(p.dh0 + (size_t)bb * p.HD + ch) = c;
+    if (tile == 0 && warp == 0) *reinterpret_cast<float2*>(p.dh0 + (size_t)now.bb * p.HD + ch) = c;
     __syncwarp();
     prefetch_vw(next);
-#pragma unroll
-    for (int r = 0; r < kRows; ++r) {
-      a[r] = na[r];
-      d[r] = nd[r];
-    }
     now = next;
     next = later;
+    side ^= 1;
+    return now.k >= 0;
+  };
+  // (Two register sets in turn spill here: 263 us instead of 224 for B8 T8192 H6
+  // D128 float32.)
+  while (turn(std::integral_constant<int, 0>{})) {
+#pragma unroll
+    for (int r = 0; r < kRows; ++r) {
+      a[0][r] = a[1][r];
+      d[0][r] = d[1][r];
+    }
   }
 }
 
