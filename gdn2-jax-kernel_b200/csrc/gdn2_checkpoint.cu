@@ -17,8 +17,8 @@ namespace {
 constexpr int kMaxTensors = GDN2_INT8_MAX_TENSORS;
 struct Tensors {
   const void* x[kMaxTensors];   // values (pack: source, unpack: destination)
-  const void* c[kMaxTensors];   // codes
-  const void* s[kMaxTensors];   // scales
+  int8_t* codes;                // of all, one tensor after another
+  float* scales;
 };
 
 // E values of one thread, 16 bytes of T.
@@ -128,8 +128,8 @@ template <typename T>
 __global__ void __launch_bounds__(256) k_pack(Tensors a, size_t n) {
   constexpr int E = Vec<T>::E;
   const T* x = static_cast<const T*>(a.x[blockIdx.y]);
-  int8_t* c = static_cast<int8_t*>(const_cast<void*>(a.c[blockIdx.y]));
-  float* s = static_cast<float*>(const_cast<void*>(a.s[blockIdx.y]));
+  int8_t* c = a.codes + blockIdx.y * n;
+  float* s = a.scales + blockIdx.y * (n / kGroup);
   const size_t base = (size_t)blockIdx.x * (256 * E * kUnroll) + threadIdx.x * E;
   float v[kUnroll][E] = {};
 #pragma unroll
@@ -152,8 +152,8 @@ template <typename T>
 __global__ void __launch_bounds__(256) k_unpack(Tensors a, size_t n) {
   constexpr int E = Vec<T>::E;
   T* x = static_cast<T*>(const_cast<void*>(a.x[blockIdx.y]));
-  const int8_t* c = static_cast<const int8_t*>(a.c[blockIdx.y]);
-  const float* s = static_cast<const float*>(a.s[blockIdx.y]);
+  const int8_t* c = a.codes + blockIdx.y * n;
+  const float* s = a.scales + blockIdx.y * (n / kGroup);
   const size_t base = (size_t)blockIdx.x * (256 * E * kUnroll) + threadIdx.x * E;
   unsigned w[kUnroll][E / 4] = {};
   float scale[kUnroll] = {};
@@ -249,9 +249,8 @@ unsigned blocks_for(size_t n, int elem_bytes) {
 }
 
 // The checks that pack and unpack share; fills `a`.
-int check_tensors(const char* what, int dtype, int n_tensors, void* const* values,
-                  void* const* codes, float* const* scales, size_t n, Tensors& a) {
-  (void)what;
+int check_tensors(int dtype, int n_tensors, const void* const* values, const void* codes,
+                  const float* scales, size_t n, Tensors& a) {
   if (dtype != GDN2_F32 && dtype != GDN2_BF16)
     return report_error(GDN2_ERR_INVALID, "gdn2_int8: unsupported dtype code");
   if (n_tensors < 1 || n_tensors > kMaxTensors)
@@ -260,15 +259,16 @@ int check_tensors(const char* what, int dtype, int n_tensors, void* const* value
     return report_error(GDN2_ERR_INVALID, "gdn2_int8: a positive multiple of 64 values per tensor");
   if (!values || !codes || !scales)
     return report_error(GDN2_ERR_INVALID, "gdn2_int8: null buffer pointer");
+  if (!aligned16(codes) || ((uintptr_t)scales & 3))
+    return report_error(GDN2_ERR_INVALID, "gdn2_int8: values and codes must be 16-byte aligned");
   for (int i = 0; i < n_tensors; ++i) {
-    if (!values[i] || !codes[i] || !scales[i])
-      return report_error(GDN2_ERR_INVALID, "gdn2_int8: null buffer pointer");
-    if (!aligned16(values[i]) || !aligned16(codes[i]) || ((uintptr_t)scales[i] & 3))
+    if (!values[i]) return report_error(GDN2_ERR_INVALID, "gdn2_int8: null buffer pointer");
+    if (!aligned16(values[i]))
       return report_error(GDN2_ERR_INVALID, "gdn2_int8: values and codes must be 16-byte aligned");
     a.x[i] = values[i];
-    a.c[i] = codes[i];
-    a.s[i] = scales[i];
   }
+  a.codes = static_cast<int8_t*>(const_cast<void*>(codes));
+  a.scales = const_cast<float*>(scales);
   return GDN2_OK;
 }
 
@@ -295,11 +295,10 @@ int launched() {
 
 using namespace gdn2;
 
-extern "C" int gdn2_int8_pack(int dtype, int n_tensors, const void* const* values,
-                              void* const* codes, float* const* scales, size_t n, void* stream) {
+extern "C" int gdn2_int8_pack(int dtype, int n_tensors, const void* const* values, void* codes,
+                              float* scales, size_t n, void* stream) {
   Tensors a{};
-  const int rc = check_tensors("pack", dtype, n_tensors, const_cast<void* const*>(values), codes,
-                               scales, n, a);
+  const int rc = check_tensors(dtype, n_tensors, values, codes, scales, n, a);
   if (rc) return rc;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   if (dtype == GDN2_F32)
@@ -309,13 +308,10 @@ extern "C" int gdn2_int8_pack(int dtype, int n_tensors, const void* const* value
   return launched();
 }
 
-extern "C" int gdn2_int8_unpack(int dtype, int n_tensors, void* const* values,
-                                const void* const* codes, const float* const* scales, size_t n,
-                                void* stream) {
+extern "C" int gdn2_int8_unpack(int dtype, int n_tensors, void* const* values, const void* codes,
+                                const float* scales, size_t n, void* stream) {
   Tensors a{};
-  const int rc = check_tensors("unpack", dtype, n_tensors, values,
-                               const_cast<void* const*>(codes), const_cast<float* const*>(scales),
-                               n, a);
+  const int rc = check_tensors(dtype, n_tensors, values, codes, scales, n, a);
   if (rc) return rc;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   if (dtype == GDN2_F32)

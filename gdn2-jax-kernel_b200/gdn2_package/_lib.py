@@ -9,6 +9,8 @@ from __future__ import annotations
 import ctypes
 import os
 
+import torch
+
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_HERE, "libgdn2.so")
 
@@ -156,32 +158,19 @@ def load():
     return lib
 
 
-def raw_stream(index):
-    """cudaStream_t of the current stream of CUDA device ``index``."""
-    import torch
-    get = getattr(torch._C, "_cuda_getCurrentRawStream", None)   # 2 us less than the object
-    return get(index) if get else torch.cuda.current_stream(index).cuda_stream
+# cudaStream_t of the current stream of a CUDA device index (the public object
+# costs 2 us more)
+raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
+    lambda index: torch.cuda.current_stream(index).cuda_stream)
 
 
-class on_device:
-    """``torch.cuda.device`` for a device index, without its cost where that
-    device is the current one."""
-
-    __slots__ = ("index", "outer")
-
-    def __init__(self, index):
-        self.index = index
-
-    def __enter__(self):
-        import torch
-        self.outer = None
-        if torch.cuda.current_device() != self.index:
-            self.outer = torch.cuda.device(self.index)
-            self.outer.__enter__()
-
-    def __exit__(self, *exc):
-        if self.outer is not None:
-            self.outer.__exit__(*exc)
+def on_device(index, fn, *args):
+    """``fn(*args)`` with CUDA device ``index`` current (``torch.cuda.device``
+    without its cost where it is already)."""
+    if torch.cuda.current_device() == index:
+        return fn(*args)
+    with torch.cuda.device(index):
+        return fn(*args)
 
 
 def check(rc, what):

@@ -60,23 +60,18 @@ class Gdn2Checkpoint:
         return sum(c.numel() + 4 * s.numel() for _, c, s in self.buffers)
 
 
-def _pointers(ps):
-    return (ctypes.c_void_p * len(ps))(*ps)
+_ARRAYS = [ctypes.c_void_p * n for n in range(_MAX_TENSORS + 1)]
 
 
 def _launches(dtypes, counts):
     """Indexes of the tensors of each launch: one type and size, at most eight."""
+    if len(dtypes) <= _MAX_TENSORS and len(set(dtypes)) == 1 and len(set(counts)) == 1:
+        return [((dtypes[0], counts[0]), list(range(len(dtypes))))]
     sets = {}
     for i, key in enumerate(zip(dtypes, counts)):
         sets.setdefault(key, []).append(i)
     return [(key, at[i:i + _MAX_TENSORS]) for key, at in sets.items()
             for i in range(0, len(at), _MAX_TENSORS)]
-
-
-def _buffer_pointers(at, codes, scales, n):
-    c, s = codes.data_ptr(), scales.data_ptr()
-    return (_pointers([c + j * n for j in range(len(at))]),
-            _pointers([s + j * (n // GROUP * 4) for j in range(len(at))]))
 
 
 def gdn2_checkpoint_pack(*tensors):
@@ -85,44 +80,43 @@ def gdn2_checkpoint_pack(*tensors):
     ts = [t if isinstance(t, torch.Tensor) else torch.as_tensor(t) for t in tensors]
     if not ts:
         raise _fwd.Gdn2ShapeError("no tensors to pack")
-    for t in ts:
-        if not t.dtype.is_floating_point:
+    shapes, dtypes, sizes = [t.shape for t in ts], [t.dtype for t in ts], [t.numel() for t in ts]
+    for shape, dt, n in zip(shapes, dtypes, sizes):
+        if not dt.is_floating_point:
             raise _fwd.Gdn2ShapeError("inputs must be floating point")
-        if t.dim() == 0 or t.shape[-1] % GROUP or t.numel() == 0:
+        if not n or not shape or shape[-1] % GROUP:
             raise _fwd.Gdn2ShapeError(
-                f"the last axis must be a positive multiple of {GROUP}; got {tuple(t.shape)}")
+                f"the last axis must be a positive multiple of {GROUP}; got {tuple(shape)}")
     on_host = not ts[0].is_cuda
     dev = torch.device("cuda", torch.cuda.current_device()) if on_host else ts[0].device
-    x = [_operand(t, dev, t.dtype if t.dtype is torch.bfloat16 else torch.float32) for t in ts]
-    lib = _lib.load()
+    kinds = [torch.bfloat16 if dt is torch.bfloat16 else torch.float32 for dt in dtypes]
+    x = [_operand(t, dev, dt) for t, dt in zip(ts, kinds)]
+    pack, stream = _lib.load().gdn2_int8_pack, _lib.raw_stream(dev.index)
     buffers = []
-    with _lib.on_device(dev.index):
-        stream = _lib.raw_stream(dev.index)
-        for (dt, n), at in _launches([t.dtype for t in x], [t.numel() for t in x]):
-            codes = torch.empty((len(at), n), dtype=torch.int8, device=dev)
-            scales = torch.empty((len(at), n // GROUP), dtype=torch.float32, device=dev)
-            rc = lib.gdn2_int8_pack(_lib.BF16 if dt is torch.bfloat16 else _lib.F32, len(at),
-                                    _pointers([x[i].data_ptr() for i in at]),
-                                    *_buffer_pointers(at, codes, scales, n), n, stream)
-            _lib.check(rc, "gdn2_checkpoint_pack")
-            buffers.append((at, codes, scales))
-    return Gdn2Checkpoint(buffers, [t.shape for t in ts], [t.dtype for t in ts], on_host)
+    for (dt, n), at in _launches(kinds, sizes):
+        codes = torch.empty((len(at), n), dtype=torch.int8, device=dev)
+        scales = torch.empty((len(at), n // GROUP), dtype=torch.float32, device=dev)
+        rc = _lib.on_device(dev.index, pack, _lib.BF16 if dt is torch.bfloat16 else _lib.F32,
+                            len(at), _ARRAYS[len(at)](*[x[i].data_ptr() for i in at]),
+                            codes.data_ptr(), scales.data_ptr(), n, stream)
+        _lib.check(rc, "gdn2_checkpoint_pack")
+        buffers.append((at, codes, scales))
+    return Gdn2Checkpoint(buffers, shapes, dtypes, on_host)
 
 
 def gdn2_checkpoint_unpack(kept):
     """The tensors that ``kept`` holds, each in the type it was packed from."""
     dev = kept.buffers[0][1].device
-    out = [torch.empty(s, dtype=dt if dt is torch.bfloat16 else torch.float32, device=dev)
-           for s, dt in zip(kept.shapes, kept.dtypes)]
-    lib = _lib.load()
-    with _lib.on_device(dev.index):
-        stream = _lib.raw_stream(dev.index)
-        for at, codes, scales in kept.buffers:
-            n = codes.shape[1]
-            rc = lib.gdn2_int8_unpack(
-                _lib.BF16 if out[at[0]].dtype is torch.bfloat16 else _lib.F32, len(at),
-                _pointers([out[i].data_ptr() for i in at]),
-                *_buffer_pointers(at, codes, scales, n), n, stream)
-            _lib.check(rc, "gdn2_checkpoint_unpack")
+    unpack, stream = _lib.load().gdn2_int8_unpack, _lib.raw_stream(dev.index)
+    out = [None] * len(kept.shapes)
+    for at, codes, scales in kept.buffers:
+        bf16 = kept.dtypes[at[0]] is torch.bfloat16
+        kind = torch.bfloat16 if bf16 else torch.float32
+        for i in at:
+            out[i] = scales.new_empty(kept.shapes[i], dtype=kind)
+        rc = _lib.on_device(dev.index, unpack, _lib.BF16 if bf16 else _lib.F32, len(at),
+                            _ARRAYS[len(at)](*[out[i].data_ptr() for i in at]),
+                            codes.data_ptr(), scales.data_ptr(), codes.shape[1], stream)
+        _lib.check(rc, "gdn2_checkpoint_unpack")
     out = [t if t.dtype is dt else t.to(dt) for t, dt in zip(out, kept.dtypes)]
     return tuple(t.cpu() for t in out) if kept.on_host else tuple(out)

@@ -17,6 +17,8 @@ sanitiser acts: a clip inside the recurrence would make it serial.
 """
 from __future__ import annotations
 
+import functools
+
 import torch
 
 from . import _lib
@@ -115,13 +117,19 @@ def _int8_pointers(packed):
     return c, s, c + n, s + n // GROUP * 4
 
 
-def _workspace(lib, shape, dev):
+@functools.lru_cache(maxsize=256)
+def _workspace_bytes(B, T, H, D):
+    n = _lib.load().gdn2_recur_workspace_bytes(B, T, H, D)
+    if n == 0:
+        raise _fwd.Gdn2ShapeError("invalid sizes for the workspace")
+    return n
+
+
+def _workspace(shape, dev):
     """Scratch of one call; none where the sequence is one tile."""
     if shape[1] <= INTERVAL:
         return None, 0
-    n = lib.gdn2_recur_workspace_bytes(*shape)
-    if n == 0:
-        raise _fwd.Gdn2ShapeError("invalid sizes for the workspace")
+    n = _workspace_bytes(*shape)
     return torch.empty(n, dtype=torch.uint8, device=dev), n
 
 
@@ -129,22 +137,21 @@ def _forward(c, keep, int8):
     lib = _lib.load()
     B, T, H, D, dev = c.B, c.T, c.H, c.D, c.dev
     o = torch.empty_like(c.v, dtype=torch.float32)
-    hf = torch.empty((B, H, D), dtype=torch.float32, device=dev)
+    hf = o.new_empty((B, H, D))
     kept = packed = None
     if keep:
-        kept = torch.empty((B, -(-T // INTERVAL), H, D), dtype=torch.float32, device=dev)
+        kept = o.new_empty((B, -(-T // INTERVAL), H, D))
         if int8:
             packed = (torch.empty((2, B, T, H, D), dtype=torch.int8, device=dev),
-                      torch.empty((2, B, T, H, D // GROUP), dtype=torch.float32, device=dev))
-    with _lib.on_device(dev.index):
-        ws, n = _workspace(lib, (B, T, H, D), dev)
-        stream = _lib.raw_stream(dev.index)
-        rc = lib.gdn2_recur_fwd(c.code, c.v.data_ptr(), c.w.data_ptr(), c.g.data_ptr(), _ptr(c.h0),
-                                o.data_ptr(), hf.data_ptr(), _ptr(kept), *_int8_pointers(packed),
-                                _ptr(ws), n, B, T, H, D, stream)
-        _lib.check(rc, "gdn2_linear_recurrence")
-        if ws is not None:
-            _lib.check_status(ws, stream, "gdn2_linear_recurrence", synced=c.on_host)
+                      o.new_empty((2, B, T, H, D // GROUP)))
+    ws, n = _workspace((B, T, H, D), dev)
+    stream = _lib.raw_stream(dev.index)
+    rc = _lib.on_device(dev.index, lib.gdn2_recur_fwd, c.code, c.v.data_ptr(), c.w.data_ptr(),
+                        c.g.data_ptr(), _ptr(c.h0), o.data_ptr(), hf.data_ptr(), _ptr(kept),
+                        *_int8_pointers(packed), _ptr(ws), n, B, T, H, D, stream)
+    _lib.check(rc, "gdn2_linear_recurrence")
+    if ws is not None:
+        _lib.check_status(ws, stream, "gdn2_linear_recurrence", synced=c.on_host)
     return o, hf, (Gdn2RecurrenceResiduals(c, packed, kept) if keep else None)
 
 
@@ -190,17 +197,16 @@ def gdn2_linear_recurrence_backward(residuals, dout, dh_final=None):
         dh = _operand(dh_final, dev, torch.float32)
     lib = _lib.load()
     dv, dw, dg = torch.empty_like(r.g), torch.empty_like(r.g), torch.empty_like(r.g)
-    dh0 = torch.empty((B, H, D), dtype=torch.float32, device=dev)
-    with _lib.on_device(dev.index):
-        ws, n = _workspace(lib, r.shape, dev)
-        stream = _lib.raw_stream(dev.index)
-        rc = lib.gdn2_recur_bwd(r.code, _ptr(r.v), _ptr(r.w), r.g.data_ptr(),
-                                *_int8_pointers(r.int8), r.kept.data_ptr(), do.data_ptr(),
-                                _ptr(dh), dv.data_ptr(), dw.data_ptr(), dg.data_ptr(),
-                                dh0.data_ptr(), _ptr(ws), n, B, T, H, D, stream)
-        _lib.check(rc, "gdn2_linear_recurrence_backward")
-        if ws is not None:
-            _lib.check_status(ws, stream, "gdn2_linear_recurrence_backward", synced=r.on_host)
+    dh0 = do.new_empty((B, H, D))
+    ws, n = _workspace(r.shape, dev)
+    stream = _lib.raw_stream(dev.index)
+    rc = _lib.on_device(dev.index, lib.gdn2_recur_bwd, r.code, _ptr(r.v), _ptr(r.w),
+                        r.g.data_ptr(), *_int8_pointers(r.int8), r.kept.data_ptr(), do.data_ptr(),
+                        _ptr(dh), dv.data_ptr(), dw.data_ptr(), dg.data_ptr(), dh0.data_ptr(),
+                        _ptr(ws), n, B, T, H, D, stream)
+    _lib.check(rc, "gdn2_linear_recurrence_backward")
+    if ws is not None:
+        _lib.check_status(ws, stream, "gdn2_linear_recurrence_backward", synced=r.on_host)
     out = [t if t.dtype is dt else t.to(dt)
            for t, dt in zip((dv, dw, dg, dh0), (*r.dtypes, r.h0_dtype or torch.float32))]
     return tuple(t.cpu() for t in out) if r.on_host else tuple(out)

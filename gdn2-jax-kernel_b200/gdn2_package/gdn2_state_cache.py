@@ -119,10 +119,10 @@ def gdn2_state_write(cache, h, slots=None):
     B, S = h.shape[0], cache.slots
     at, _ = _slots(slots, B, S, dev, "slots", True)
     hs = _operand(h, dev, torch.float32)
-    with _lib.on_device(dev.index):
-        rc = _lib.load().gdn2_state_write(hs.data_ptr(), _ptr(at), cache.codes.data_ptr(),
-                                          cache.scales.data_ptr(), B, S, cache.H, cache.D,
-                                          float(_fwd.CLIP), _lib.raw_stream(dev.index))
+    _, H, D, _ = h.shape
+    rc = _lib.on_device(dev.index, _lib.load().gdn2_state_write, hs.data_ptr(), _ptr(at),
+                        cache.codes.data_ptr(), cache.scales.data_ptr(), B, S, H, D,
+                        float(_fwd.CLIP), _lib.raw_stream(dev.index))
     _lib.check(rc, "gdn2_state_write")
 
 
@@ -132,16 +132,16 @@ def gdn2_state_read(cache, slots=None, dtype=torch.float32):
     dev = _on_gpu(cache)
     if dtype not in (torch.float32, torch.bfloat16):
         raise _fwd.Gdn2ShapeError(f"dtype must be float32 or bfloat16; got {dtype}")
-    S, H, D = cache.slots, cache.H, cache.D
+    S, H, D, _ = cache.codes.shape
     B = S if slots is None else len(slots)
     if B == 0:
         raise _fwd.Gdn2ShapeError("empty problem")
     at, _ = _slots(slots, B, S, dev, "slots", False)
-    h = torch.empty((B, H, D, D), dtype=dtype, device=dev)
-    with _lib.on_device(dev.index):
-        rc = _lib.load().gdn2_state_read(_lib.F32 if dtype == torch.float32 else _lib.BF16,
-                                         cache.codes.data_ptr(), cache.scales.data_ptr(), _ptr(at),
-                                         h.data_ptr(), B, S, H, D, _lib.raw_stream(dev.index))
+    h = cache.scales.new_empty((B, H, D, D), dtype=dtype)
+    rc = _lib.on_device(dev.index, _lib.load().gdn2_state_read,
+                        _lib.F32 if dtype is torch.float32 else _lib.BF16, cache.codes.data_ptr(),
+                        cache.scales.data_ptr(), _ptr(at), h.data_ptr(), B, S, H, D,
+                        _lib.raw_stream(dev.index))
     _lib.check(rc, "gdn2_state_read")
     return h
 
@@ -167,8 +167,10 @@ def gdn2_decode_cached(q, k, v, w, b, g, scale, cache, slots=None, out_slots=Non
         raise _fwd.Gdn2ShapeError(f"head dim D={D} unsupported (64 or 128)")
     if B * T * H == 0:
         raise _fwd.Gdn2ShapeError("empty problem")
-    if any(not t.dtype.is_floating_point for t in ts):
-        raise _fwd.Gdn2ShapeError("inputs must be floating point")
+    dtypes = [t.dtype for t in ts]
+    for dt in dtypes:
+        if not dt.is_floating_point:
+            raise _fwd.Gdn2ShapeError("inputs must be floating point")
     if cache.codes.shape[1:3] != (H, D):
         raise _fwd.Gdn2ShapeError(f"the cache holds states of H={cache.H}, D={cache.D}; "
                                   f"got H={H}, D={D}")
@@ -185,17 +187,16 @@ def gdn2_decode_cached(q, k, v, w, b, g, scale, cache, slots=None, out_slots=Non
                 readers.setdefault(s, []).append(i)
             if any(d >= 0 and any(j != i for j in readers.get(d, ())) for i, d in enumerate(dst_host)):
                 raise _fwd.Gdn2ShapeError("a slot of out_slots is another row's slot")
-    bf16 = all(t.dtype is torch.bfloat16 for t in ts)
+    bf16 = dtypes.count(torch.bfloat16) == 6
     cdt = torch.bfloat16 if bf16 else torch.float32
-    x = [_operand(t, dev, cdt) for t in ts]
-    o = torch.empty(shape, dtype=torch.float32, device=dev)
+    x = [_operand(t, dev, cdt) for t in ts]   # copies live until the launch
+    o = cache.scales.new_empty(shape)
     code = _lib.BF16 if bf16 else _lib.F32
     if _fwd.GATES == "raw":
         code |= _lib.GATES_RAW
-    with _lib.on_device(dev.index):
-        rc = _lib.load().gdn2_decode_cached(
-            code, *[t.data_ptr() for t in x], cache.codes.data_ptr(), cache.scales.data_ptr(),
-            _ptr(src), _ptr(dst), o.data_ptr(), B, T, H, D, S, float(scale), float(_fwd.CLIP),
-            _lib.raw_stream(dev.index))
+    rc = _lib.on_device(dev.index, _lib.load().gdn2_decode_cached, code,
+                        *[t.data_ptr() for t in x], cache.codes.data_ptr(), cache.scales.data_ptr(), _ptr(src), _ptr(dst),
+                        o.data_ptr(), B, T, H, D, S, float(scale), float(_fwd.CLIP),
+                        _lib.raw_stream(dev.index))
     _lib.check(rc, "gdn2_decode_cached")
     return o if ts[0].is_cuda else o.cpu()

@@ -248,19 +248,19 @@ int gdn2_decode(int dtype, const void* q, const void* k, const void* v, const vo
  * 64 consecutive values share one float32 scale; code = rint(127 x / max|x|)
  * with ties to even, decided exactly, scale = max|x| / 127, value = code *
  * scale (off by at most max|x| / 254).  A group whose largest |x| is below
- * 2^-100 is stored as zeros; one that holds a NaN or an infinity gets a NaN
+ * 2^-100 reads back as zeros; one that holds a NaN or an infinity gets a NaN
  * scale and reads back as NaN throughout.  Values and codes are 16-byte
  * aligned.  No counterpart in the reference.
  *
  * Pack / unpack n_tensors tensors (1 .. GDN2_INT8_MAX_TENSORS) of n values each
- * (a multiple of 64) in one launch: values[i] of `dtype`, codes[i] n int8,
- * scales[i] n / 64 float32.  The pointer arrays are host arrays, read before
- * the call returns. */
+ * (a multiple of 64) in one launch: values[i] of `dtype`; codes (n_tensors, n)
+ * int8 and scales (n_tensors, n / 64) float32 hold one tensor after another.
+ * `values` is a host array, read before the call returns. */
 #define GDN2_INT8_MAX_TENSORS 8
-int gdn2_int8_pack(int dtype, int n_tensors, const void* const* values, void* const* codes,
-                   float* const* scales, size_t n, void* stream);
-int gdn2_int8_unpack(int dtype, int n_tensors, void* const* values, const void* const* codes,
-                     const float* const* scales, size_t n, void* stream);
+int gdn2_int8_pack(int dtype, int n_tensors, const void* const* values, void* codes,
+                   float* scales, size_t n, void* stream);
+int gdn2_int8_unpack(int dtype, int n_tensors, void* const* values, const void* codes,
+                     const float* scales, size_t n, void* stream);
 
 /* int8 cache of recurrent states: codes (S, H, D, D) int8 and scales
  * (S, H, D, D / 64) float32 hold one state per slot.  Row b of a call uses slot

@@ -69,6 +69,25 @@ def test_ties_and_their_neighbours():
     assert c[:4].tolist() == [0, 2, 2, 4]
 
 
+@pytest.mark.parametrize("power", [-90, 0, 119])
+def test_every_bf16_quotient_next_to_a_half(power):
+    """All pairs of 8-bit mantissas, sizes down to 2^-9 of the largest: the codes
+    of a bf16 group are the correctly rounded ones, ties (one pair in a few
+    hundred) included."""
+    top = torch.arange(128, 256).view(-1, 1, 1)
+    x = torch.arange(128, 256).view(1, -1, 1) * 0.5 ** torch.arange(0, 10).view(1, 1, -1)
+    x = x.reshape(1, -1).expand(128, -1).clone()
+    x[x > top[:, 0]] *= 0.5
+    x[:, ::2] *= -1
+    x = torch.nn.functional.pad(x, (0, -x.shape[1] % 63)).view(128, -1, 63)
+    x = torch.cat([x, top.expand(-1, x.shape[1], 1)], 2) * 2.0 ** power
+    x = x.to(torch.bfloat16).cuda()
+    assert torch.isfinite(x).all()
+    kept = gdn2_checkpoint_pack(x)
+    codes, scales = pack64(x)
+    assert torch.equal(kept.codes[0].long(), codes) and torch.equal(kept.scales[0], scales)
+
+
 def test_zero_tiny_and_non_finite_groups():
     x = torch.randn(7, 64, generator=torch.Generator().manual_seed(3)).cuda()
     x[1] = 0

@@ -21,15 +21,17 @@ def test_int8_entry_points_refuse():
     lib = _lib.load()
     bad = _lib.ERR_INVALID
     for fn in (lib.gdn2_int8_pack, lib.gdn2_int8_unpack):
-        assert fn(7, 1, arr(P), arr(P), arr(P), 64, None) == bad       # dtype
-        assert fn(0, 0, arr(P), arr(P), arr(P), 64, None) == bad       # no tensors
-        assert fn(0, 9, arr(*[P] * 9), arr(*[P] * 9), arr(*[P] * 9), 64, None) == bad
-        assert fn(0, 1, arr(P), arr(P), arr(P), 0, None) == bad
-        assert fn(0, 1, arr(P), arr(P), arr(P), 65, None) == bad       # not a multiple of 64
-        assert fn(0, 1, None, arr(P), arr(P), 64, None) == bad
-        assert fn(0, 2, arr(P, None), arr(P, P), arr(P, P), 64, None) == bad
-        assert fn(0, 1, arr(ODD), arr(P), arr(P), 64, None) == bad     # alignment
-        assert fn(0, 1, arr(P), arr(ODD), arr(P), 64, None) == bad
+        assert fn(7, 1, arr(P), P, P, 64, None) == bad            # dtype
+        assert fn(0, 0, arr(P), P, P, 64, None) == bad            # no tensors
+        assert fn(0, 9, arr(*[P] * 9), P, P, 64, None) == bad
+        assert fn(0, 1, arr(P), P, P, 0, None) == bad
+        assert fn(0, 1, arr(P), P, P, 65, None) == bad            # not a multiple of 64
+        assert fn(0, 1, None, P, P, 64, None) == bad
+        assert fn(0, 1, arr(P), None, P, 64, None) == bad
+        assert fn(0, 1, arr(P), P, None, 64, None) == bad
+        assert fn(0, 2, arr(P, None), P, P, 64, None) == bad
+        assert fn(0, 1, arr(ODD), P, P, 64, None) == bad          # alignment
+        assert fn(0, 1, arr(P), ODD, P, 64, None) == bad
         assert b"aligned" in lib.gdn2_last_error()
 
 
