@@ -3,9 +3,13 @@
 // gdn2_int8.cuh applied as values are stored and taken off as they are read.
 //
 // Every kernel moves each byte once and is bound by HBM: float32 values take
-// 4 + 1.0625 bytes either way.  A thread holds 16 bytes of values (4 float32 or
-// 8 bf16), so a group of 64 is 16 or 8 neighbouring lanes, whose maximum takes
-// 4 or 3 shuffles, and the codes of a warp leave as one contiguous store.
+// 4 + 1.0625 bytes either way.  A thread holds four pieces of 16 bytes of values
+// (4 float32 or 8 bf16), so a group of 64 is 16 or 8 neighbouring lanes, whose
+// maximum takes 4 or 3 shuffles, and the codes of a warp leave as one contiguous
+// store.  Five tensors of 50.3M values, of the measured copy rate: float32 packed
+// in 197 us (99%) and restored in 193 us (101%), bf16 in 136 us (86%) and 119 us
+// (99%).  States of 256 x 8 heads of 128 are written in 28.7 us (90%: the slots
+// are looked through first) and read in 25.3 us (102%).
 #include "../../include/gdn2.h"
 #include "gdn2_int8.cuh"
 

@@ -3,19 +3,23 @@
 // it stands there), with the state read as codes, held in float32 registers
 // over the tokens of the call and stored as codes again.
 //
-// A step is bound by the state's bytes, 2 x 17 KB a head at D = 128 against
-// 2 x 64 KB for float32 states, and close behind by the instructions of taking
-// every code apart and putting it together again.
+// A step moves 2 x 17 KB a head at D = 128, against 2 x 64 KB for float32 states.
+// What bounds it is the instructions of taking every code apart and putting it
+// together again: 17 a value, issued at 2.7 of 4 a cycle.  One token for 256 rows
+// x 8 heads of 128 takes 23.6 us, 46% of the copy rate (1024 rows: 89 us, 49%);
+// one row 4.7 us, all of it latency.  Four tokens a call take 66 us, a third less
+// than four calls.
 //
 // One CTA per (row, head).  The head's codes and scales (17 KB, contiguous) come
 // to shared memory by asynchronous copies, so the bytes in flight do not cost
-// registers and five CTAs fit an SM.  A thread works on 8 columns (one 8-byte
-// word of codes) of R key rows; the D / 8 lanes of a row sit in one warp, so the
-// maximum of a group of 64 columns takes three shuffles.  The two products with
-// the state (W^T h and qg^T h) are summed over a thread's rows, over the row
-// lanes of the warp, then over the warps in shared memory, always in the same
-// order.  A call of one token takes the codes apart twice (for the products and
-// for the update); a call of more tokens keeps float32 values in registers.
+// registers and four CTAs fit an SM (from registers, two: 35.5 us).  A thread
+// works on 8 columns (one 8-byte word of codes) of R key rows; the D / 8 lanes of
+// a row sit in one warp, so the maximum of a group of 64 columns takes three
+// shuffles.  The two products with the state (W^T h and qg^T h) are summed over a
+// thread's rows, over the row lanes of the warp, then over the warps in shared
+// memory, always in the same order.  A call of one token takes the codes apart
+// twice (for the products and for the update: 64 registers instead of 128); a
+// call of more tokens keeps float32 values.
 #include "../../include/gdn2.h"
 #include "gdn2_int8.cuh"
 
@@ -24,9 +28,6 @@ int report_error(int code, const char* msg);
 
 namespace {
 
-#ifndef MINB
-#define MINB 4
-#endif
 template <int D> struct Shape {
   static constexpr int NW = D / 16;          // warps
   static constexpr int CL = D / 8;           // lanes of a row
@@ -73,7 +74,7 @@ __device__ __forceinline__ void update8(float2 (&x)[4], float d, float kg, const
 }
 
 template <typename T, int D, bool ONE>
-__global__ void __launch_bounds__(Shape<D>::NW * 32, D == 64 ? 6 : ONE ? MINB : 2)
+__global__ void __launch_bounds__(Shape<D>::NW * 32, D == 64 ? 6 : ONE ? 4 : 2)
 k_decode_cached(const T* __restrict__ q, const T* __restrict__ k, const T* __restrict__ v,
                 const T* __restrict__ w, const T* __restrict__ b, const T* __restrict__ g,
                 int8_t* codes, float* scales, const int* __restrict__ src,

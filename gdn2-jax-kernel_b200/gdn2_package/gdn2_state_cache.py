@@ -133,9 +133,13 @@ def gdn2_state_read(cache, slots=None, dtype=torch.float32):
     if dtype not in (torch.float32, torch.bfloat16):
         raise _fwd.Gdn2ShapeError(f"dtype must be float32 or bfloat16; got {dtype}")
     S, H, D, _ = cache.codes.shape
-    B = S if slots is None else len(slots)
-    if B == 0:
-        raise _fwd.Gdn2ShapeError("empty problem")
+    B = S
+    if slots is not None:
+        if not isinstance(slots, torch.Tensor):
+            slots = torch.as_tensor(slots)
+        B = slots.numel()
+        if B == 0:
+            raise _fwd.Gdn2ShapeError("empty problem")
     at, _ = _slots(slots, B, S, dev, "slots", False)
     h = cache.scales.new_empty((B, H, D, D), dtype=dtype)
     rc = _lib.on_device(dev.index, _lib.load().gdn2_state_read,
@@ -195,8 +199,8 @@ def gdn2_decode_cached(q, k, v, w, b, g, scale, cache, slots=None, out_slots=Non
     if _fwd.GATES == "raw":
         code |= _lib.GATES_RAW
     rc = _lib.on_device(dev.index, _lib.load().gdn2_decode_cached, code,
-                        *[t.data_ptr() for t in x], cache.codes.data_ptr(), cache.scales.data_ptr(), _ptr(src), _ptr(dst),
-                        o.data_ptr(), B, T, H, D, S, float(scale), float(_fwd.CLIP),
-                        _lib.raw_stream(dev.index))
+                        *[t.data_ptr() for t in x], cache.codes.data_ptr(),
+                        cache.scales.data_ptr(), _ptr(src), _ptr(dst), o.data_ptr(), B, T, H, D, S,
+                        float(scale), float(_fwd.CLIP), _lib.raw_stream(dev.index))
     _lib.check(rc, "gdn2_decode_cached")
     return o if ts[0].is_cuda else o.cpu()

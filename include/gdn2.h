@@ -293,7 +293,9 @@ int gdn2_decode_cached(int dtype, const void* q, const void* k, const void* v, c
  *   h_t = e^{g_t} h_{t-1} + w_t v_t,  o_t = h_t
  * on v, w, g (B, T, H, D) of `dtype` (GDN2_GATES_RAW as above), states
  * (B, H, D) float32, o float32; any T >= 1, D 64, 128 or 256, no sanitiser.
- * g may be -inf (the state restarts).  Buffers are 16-byte aligned.
+ * g is at most 0 and may be -inf (the state restarts there); a positive gate is
+ * computed as well while the products of decays over 1024 tokens stay in
+ * float32's range.  Values are 16-byte aligned, scales 4-byte.
  *
  * gdn2_recur_fwd: h0 may be NULL (zero).  `kept` (NULL: none) receives the
  * gdn2_recur_kept_floats() floats that the backward needs: the state before

@@ -32,10 +32,13 @@ def linrec64(v, w, g, h0, dout=None, dh=None, v8=None, w8=None, raw=False):
     gradients.  Beside each output the size its float32 error is counted in.
 
     An output is a sum over k of |x_{t-k}| times k decays.  Every decay carries
-    4 roundings at most (expf or 1 / (1 + expf) and a product), every join of
-    two maps 2 more; there are k / 8 + 14 joins on the way at most.  So the
-    term is off by (4 k + k / 4 + 28 + 4) U <= 32 (k + 1) U of its size, and
-    N_t = a N_{t-1} + M_t, M_t = a M_{t-1} + |x_t| sums (k + 1) times the terms."""
+    2^-22 = 4 U of its exponential and 1 U of a product, every join of two maps
+    2 U; there are k / 8 + 26 joins on the way at most, none for k = 0.  So the
+    term is off by (5 k + k / 4 + 52 + 4) U <= 32 (k + 1) U of its size (k = 1:
+    61 of 64; k = 0: 4 of 32), and N_t = a N_{t-1} + M_t, M_t = a M_{t-1} + |x_t|
+    sums (k + 1) times the terms.  An exponential is off by 2 |g| U more: what
+    is left of 32 (k + 1) covers that for g above -13 from k = 2 on, and a term
+    one token back of such a g weighs under e^-1.5 of its 2 |g| U."""
     v, w, g = v.double(), w.double(), g.double()
     B, T, H, D = v.shape
     h0 = torch.zeros((B, H, D), dtype=torch.float64, device=v.device) if h0 is None else h0.double()

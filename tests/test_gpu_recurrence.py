@@ -176,6 +176,70 @@ def test_gradients_against_differences():
                 break
 
 
+@pytest.mark.parametrize("int8", [None, "int8"])
+def test_broadcast_leaves(int8):
+    """A gate shared by rows and tokens gets the sum of their gradients."""
+    x, do, dh = make(3, 70, 2, 64, seed=18)
+    w = x["w"][:1, :1].clone().requires_grad_(True)
+    g = x["g"][:1].clone().requires_grad_(True)
+    o, h = gdn2_linear_recurrence_trainable(x["v"], w.expand(3, 70, 2, 64), g.expand(3, 70, 2, 64),
+                                            x["h0"], checkpoint=int8)
+    dw, dg = torch.autograd.grad((o, h), (w, g), (do, dh))
+    _, _, res = gdn2_linear_recurrence_with_residuals(
+        x["v"], w.detach().expand(3, 70, 2, 64), g.detach().expand(3, 70, 2, 64), x["h0"],
+        checkpoint=int8)
+    full = gdn2_linear_recurrence_backward(res, do, dh)
+    assert torch.equal(dw, full[1].sum((0, 1), keepdim=True))
+    assert torch.equal(dg, full[2].sum(0, keepdim=True))
+
+
+@pytest.mark.parametrize("seed", range(12))
+def test_shapes_over_the_range(seed):
+    """Sizes drawn over their logarithms, every type, gate form and checkpoint."""
+    import random
+    rng = random.Random(seed)
+    log = lambda lo, hi: int(round(lo * (hi / lo) ** rng.random()))  # noqa: E731
+    B, T, H, D = log(1, 40), log(1, 1500), log(1, 9), rng.choice([64, 128, 256])
+    raw = rng.random() < 0.3
+    gdn2_fwd.GATES = "raw" if raw else "activated"
+    x, do, dh = make(B, T, H, D, rng.choice([torch.float32, torch.bfloat16]), seed=seed, raw=raw,
+                     h0=rng.random() < 0.7)
+    check(x, do, dh, rng.random() < 0.5, raw)
+
+
+def test_one_tile_for_more_chains_than_the_gpu_holds():
+    """600 x 3 groups of one tile: every CTA takes several, dealt out by index."""
+    x, do, dh = make(600, 40, 3, 64, seed=19)
+    check(x, do, dh)
+    check(x, do, dh, int8=True)
+
+
+def test_more_values_than_31_bits():
+    """2^31 values and some: the end of the last row, against the same tokens run
+    alone from the state before them."""
+    T, H, D = 2 ** 20 + 70, 32, 64
+    gen = torch.Generator(device="cuda").manual_seed(20)
+    v, w, g = (torch.empty((1, T, H, D), dtype=torch.bfloat16, device="cuda") for _ in range(3))
+    for t, lo, hi in ((v, -2, 2), (w, 0, 1), (g, -2, 0)):
+        t.uniform_(lo, hi, generator=gen)
+    o, h, res = gdn2_linear_recurrence_with_residuals(v, w, g, checkpoint="int8")
+    cut = T - 200
+    tail = [t[:, cut:].contiguous() for t in (v, w, g)]
+    before = o[:, cut - 1].contiguous()
+    want = linrec64(*tail, before)
+    assert_close(o[:, cut:], *want["o"], "o")
+    assert torch.equal(h, o[:, -1])
+    do = torch.zeros_like(o)
+    do[:, -200:].uniform_(-1, 1, generator=gen)
+    dv, dw, dg, _ = gdn2_linear_recurrence_backward(res, do)
+    # 200 is no multiple of 64: the tail's states restart elsewhere, so dv alone
+    v8, w8 = values64(tail[0]), values64(tail[1])
+    want = linrec64(*tail, before, do[:, cut:].contiguous(), None, v8, w8)
+    assert_close(dv[:, cut:], *want["dv"], "dv")
+    assert_close(dw[:, cut:], *want["dw"], "dw")
+    assert bool((dv[:, :cut - 400] == 0).all())   # e^-g sums beyond float32's smallest
+
+
 def test_strided_mixed_and_host_inputs():
     x, do, dh = make(2, 90, 2, 64, seed=13)
     o, h = gdn2_linear_recurrence(**x)

@@ -140,3 +140,37 @@ def test_host_slot_checks():
             at(s, 1, 2, "slots", False)
     with pytest.raises(bad):
         at([1, 1], 2, 2, "slots", True)
+
+
+def test_calls_run_on_the_device_of_their_tensors(monkeypatch):
+    """The device is switched for a call, and back, only where another is current."""
+    seen = []
+
+    class Switch:
+        def __init__(self, index):
+            self.index = index
+
+        def __enter__(self):
+            seen.append(self.index)
+
+        def __exit__(self, *exc):
+            seen.append("back")
+
+    monkeypatch.setattr(torch.cuda, "current_device", lambda: 0)
+    monkeypatch.setattr(torch.cuda, "device", Switch)
+    assert _lib.on_device(0, lambda a, b: a + b, 1, 2) == 3 and seen == []
+    assert _lib.on_device(1, lambda: 7) == 7 and seen == [1, "back"]
+
+
+def test_slot_arguments():
+    slots = gdn2_state_cache._slots
+    bad = gdn2_fwd.Gdn2ShapeError
+    dev = torch.device("cpu")
+    assert slots(None, 2, 2, dev, "slots", True) == (None, None)
+    t, host = slots([1, -1], 2, 2, dev, "slots", True)
+    assert t.dtype == torch.int32 and t.tolist() == host == [1, -1]
+    for s in (torch.tensor(0), torch.tensor([0.0, 1.0]), torch.tensor([True, False]), [0], [[0, 1]]):
+        with pytest.raises(bad):
+            slots(s, 2, 2, dev, "slots", True)
+    with pytest.raises(bad, match="give slots"):
+        slots(None, 3, 2, dev, "slots", True)
