@@ -7,7 +7,7 @@
 // (4 float32 or 8 bf16), so a group of 64 is 16 or 8 neighbouring lanes, whose
 // maximum takes 4 or 3 shuffles, and the codes of a warp leave as one contiguous
 // store.  Five tensors of 50.3M values, of the measured copy rate: float32 packed
-// in 197 us (99%) and restored in 193 us (101%), bf16 in 136 us (86%) and 119 us
+// in 192 us (101%) and restored in 193 us (101%), bf16 in 136 us (86%) and 119 us
 // (99%).  States of 256 x 8 heads of 128 are written in 28.7 us (90%: the slots
 // are looked through first) and read in 25.3 us (102%).
 #include "../../include/gdn2.h"
@@ -126,10 +126,12 @@ __device__ __forceinline__ bool scale_place(size_t base, size_t n, size_t& group
   return lane < kUnroll && i < n;
 }
 
+// (The argument stays in constant memory: picked from by blockIdx.y it would be
+// copied to the stack, 273 us instead of 192.)
 // blockIdx.y: tensor; n: values of each (a multiple of 64).  The bounds are
 // per thread, but a group's lanes are in or out of them together.
 template <typename T>
-__global__ void __launch_bounds__(256) k_pack(Tensors a, size_t n) {
+__global__ void __launch_bounds__(256) k_pack(const __grid_constant__ Tensors a, size_t n) {
   constexpr int E = Vec<T>::E;
   const T* x = static_cast<const T*>(a.x[blockIdx.y]);
   int8_t* c = a.codes + blockIdx.y * n;
@@ -153,7 +155,7 @@ __global__ void __launch_bounds__(256) k_pack(Tensors a, size_t n) {
 }
 
 template <typename T>
-__global__ void __launch_bounds__(256) k_unpack(Tensors a, size_t n) {
+__global__ void __launch_bounds__(256) k_unpack(const __grid_constant__ Tensors a, size_t n) {
   constexpr int E = Vec<T>::E;
   T* x = static_cast<T*>(const_cast<void*>(a.x[blockIdx.y]));
   const int8_t* c = a.codes + blockIdx.y * n;
