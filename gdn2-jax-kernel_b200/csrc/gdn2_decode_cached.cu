@@ -5,10 +5,10 @@
 //
 // A step moves 2 x 17 KB a head at D = 128, against 2 x 64 KB for float32 states.
 // What bounds it is the instructions of taking every code apart and putting it
-// together again: 17 a value, issued at 2.7 of 4 a cycle.  One token for 256 rows
-// x 8 heads of 128 takes 23.6 us, 46% of the copy rate (1024 rows: 89 us, 49%);
-// one row 4.7 us, all of it latency.  Four tokens a call take 66 us, a third less
-// than four calls.
+// together again: 16 a value, issued at 2.7 of 4 a cycle.  One token for 256 rows
+// x 8 heads of 128 takes 22.6 us, 48% of the copy rate (1024 rows: 86 us, 51%);
+// one row 4.3 us, all of it latency.  Four tokens a call take 67 us, a
+// quarter less than four calls; 16 warps a CTA made that 103 us (more partial sums).
 //
 // One CTA per (row, head).  The head's codes and scales (17 KB, contiguous) come
 // to shared memory by asynchronous copies, so the bytes in flight do not cost
@@ -132,9 +132,11 @@ k_decode_cached(const T* __restrict__ q, const T* __restrict__ k, const T* __res
     if (lane == 0) red[buf][warp] = qk;
   };
   size_t off = ((size_t)bb * T_ * H + h) * D;
+  // a token is loaded a whole token before it is put, so that nothing waits for it
   if (tid < D) {
     load(off);
     put(0);
+    if (!ONE && T_ > 1) load(off + (size_t)H * D);
   }
 
   // A destination that is another row's source or destination would make the
@@ -173,8 +175,6 @@ k_decode_cached(const T* __restrict__ q, const T* __restrict__ k, const T* __res
 
   for (int t = 0; t < (ONE ? 1 : T_); ++t, off += (size_t)H * D) {
     const int buf = ONE ? 0 : t & 1;
-    const bool more = !ONE && t + 1 < T_ && tid < D;
-    if (more) load(off + (size_t)H * D);
     float2 wa[4] = {}, qa[4] = {};
 #pragma unroll
     for (int r = 0; r < R; ++r) {
@@ -205,7 +205,10 @@ k_decode_cached(const T* __restrict__ q, const T* __restrict__ k, const T* __res
       for (int i = 0; i < 4; ++i)
         *reinterpret_cast<float4*>(&part[warp][cl * 8 + 2 * i]) =
             make_float4(wa[i].x, qa[i].x, wa[i].y, qa[i].y);
-    if (more) put(buf ^ 1);
+    if (!ONE && t + 1 < T_ && tid < D) {
+      put(buf ^ 1);
+      if (t + 2 < T_) load(off + 2 * (size_t)H * D);
+    }
     __syncthreads();
     if (tid < D) {
       float dot = 0.f, wh = 0.f, qh = 0.f;
@@ -259,7 +262,8 @@ k_decode_cached(const T* __restrict__ q, const T* __restrict__ k, const T* __res
       if constexpr (ONE) {
         const int row = row_of(r0 + j);
         const float4 z = vec[0][row];
-        codes8(word_of(row), x[j]);
+        if (j & 1) convert8(word_of(row), x[j]);   // both ways: on different pipes
+        else codes8(word_of(row), x[j]);
         update8(x[j], z.w * scale_of(row), z.z, vn);
       }
       top[j] = top8(x[j]);
@@ -284,7 +288,10 @@ k_decode_cached(const T* __restrict__ q, const T* __restrict__ k, const T* __res
       }
       m = around();
     }
-    if (cl % 8 < 4) scales[(row0 + row_of(r0 + own)) * G + cl * 8 / kGroup] = group_scale(m);
+    // (m is finite here; the scale need not be the correctly rounded quotient that
+    // packed tensors promise, and its division was 3% of the instructions)
+    if (cl % 8 < 4)
+      scales[(row0 + row_of(r0 + own)) * G + cl * 8 / kGroup] = m >= kInt8Tiny ? m * (1.f / 127.f) : 0.f;
     const float inv = group_inv(m);
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
