@@ -331,3 +331,15 @@ def test_long_sequence_of_slow_decay():
     rel = float((dv.double() - put).norm() / put.norm())
     assert rel < 1e-5, rel
     assert torch.allclose(dh0.double(), c, rtol=1e-4, atol=1e-5)
+
+
+@pytest.mark.parametrize("T", [1, 15, 16, 17, 32, 33])
+def test_few_tokens(T):
+    """The serial walk of short calls, with and without kept states, beside the
+    tiles (int8 always takes them)."""
+    x, do, dh = make(5, T, 3, 64, seed=30 + T)
+    o, h = gdn2_linear_recurrence(**x)
+    o1, h1, _ = gdn2_linear_recurrence_with_residuals(**x)
+    assert torch.equal(o, o1) and torch.equal(h, h1)
+    check(x, do, dh)
+    check(x, do, dh, int8=True)
