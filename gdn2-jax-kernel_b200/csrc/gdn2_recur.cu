@@ -15,7 +15,7 @@
 // memory, and each thread walks its tokens again from the state that reaches
 // it: every global byte moves once.  What moves bounds the float32 kernels:
 // 16 bytes a value forward, 28 backward.  The bf16 and int8 ones move less and
-// are bound by latency and issue at 16 warps an SM (60 to 130 instructions for a
+// are bound by latency and issue at 16 warps an SM (64 to 140 instructions for a
 // row of 64 channels).  Of the measured copy rate, forward / backward:
 //     B8 T8192 H6 D128    float32  133 us (92%) / 225 us (96%)
 //                         with int8 checkpoints 176 (79%) / 231 (74%)

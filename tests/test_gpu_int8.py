@@ -143,6 +143,26 @@ def test_gdn2_training_from_int8_checkpoints(D, bt, bc, dtype):
         assert rel(a, b) < 0.05, (n, rel(a, b))   # half a step is 1/254 of a group's largest
 
 
+@pytest.mark.parametrize("host", [False, True])
+def test_gdn2_int8_training_with_raw_gates_and_a_tail(host):
+    """Pre-activations are packed as they are given; T that BT does not divide;
+    leaves on the GPU or on the host."""
+    gdn2_fwd.BT, gdn2_fwd.BC, gdn2_fwd.GATES, gdn2_fwd.MASKED_TAIL = 64, 16, "raw", True
+    inp = make_inputs(1, 100, 2, 64, seed=42, h0_std=0.1)
+    gen = torch.Generator().manual_seed(43)
+    dev = "cpu" if host else "cuda"
+    args = [torch.as_tensor(inp[n]).to(dev) for n in ("q", "k", "v")]
+    args += [torch.randn(1, 100, 2, 64, generator=gen).to(dev) for _ in range(3)]
+    h0, do, dh = (torch.as_tensor(inp[n]).to(dev) for n in ("h0", "dout", "dh_final"))
+    leaves = [t.clone().requires_grad_(True) for t in (*args, h0)]
+    o, h = gdn2_pallas_forward_trainable(*leaves[:6], inp["scale"], leaves[6], checkpoint="int8")
+    got = torch.autograd.grad((o, h), leaves, (do, dh))
+    restored = [values64(t) for t in args[:5]]
+    want = gdn2_backward(*restored, args[5], inp["scale"], h0, do, dh)
+    for n, a, b in zip((*NAMES, "h0"), got, want):
+        assert a.device.type == dev and torch.equal(a, b), n
+
+
 # ---------------------------------------------------------------- state cache
 
 def states(B, H, D, seed=0):
