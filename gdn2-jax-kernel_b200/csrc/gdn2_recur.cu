@@ -182,13 +182,13 @@ __device__ __forceinline__ Map unword(ulonglong2 v) {
   return {make_float2(__uint_as_float((unsigned)v.x & 0x7fffffffu), __uint_as_float((unsigned)v.y & 0x7fffffffu)),
           make_float2(__uint_as_float((unsigned)(v.x >> 32)), __uint_as_float((unsigned)(v.y >> 32)))};
 }
-// Waits until the words at p are there in every lane, kPolls times at most; a
+// Waits until the words at p are there in every lane, `polls` polls at most; a
 // wait that runs out, here or elsewhere in the call, is in the status word and
 // ends this one too.
-__device__ Map await(const ulonglong2* p, int* status) {
+__device__ Map await(const ulonglong2* p, int* status, int polls = kPolls) {
   ulonglong2 v = peek(p);
   for (int i = 1; !__all_sync(0xffffffffu, there(v)); ++i) {
-    if (i >= kPolls || (i % 4096 == 0 && *(volatile int*)status)) {
+    if (i >= polls || (i % 4096 == 0 && *(volatile int*)status)) {
       if ((threadIdx.x & 31) == 0) atomicExch(status, 1);
       break;
     }
@@ -684,6 +684,11 @@ __global__ void __launch_bounds__(256, 2) k_recur_bwd(const Args p) {
   }
 }
 
+// One warp that waits for words that nothing publishes.
+__global__ void k_recur_timeout(const ulonglong2* words, int* status, int polls) {
+  await(words + threadIdx.x, status, polls);
+}
+
 // One CTA for every place on the GPU, or one a tile where there are fewer.
 template <typename K>
 cudaError_t launch_tiles(K kernel, size_t stage, int per_sm, const Args& p, cudaStream_t s) {
@@ -827,4 +832,17 @@ extern "C" int gdn2_recur_bwd(int dtype, const void* v, const void* w, const voi
   if (e) return e;
   return launched(dtype == GDN2_F32 ? launch<false, float>(p, from8, raw, s)
                                     : launch<false, __nv_bfloat16>(p, from8, raw, s));
+}
+
+extern "C" int gdn2_selftest_recur_timeout(void* workspace, size_t workspace_bytes, int polls,
+                                           void* stream) {
+  if (!workspace || workspace_bytes < 1024 || polls < 1)
+    return report_error(GDN2_ERR_INVALID, "gdn2_selftest_recur_timeout: bad workspace or poll count");
+  char* base = reinterpret_cast<char*>((reinterpret_cast<uintptr_t>(workspace) + 255) & ~(uintptr_t)255);
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  const cudaError_t e = cudaMemsetAsync(base, 0, 768, s);   // the header and 512 bytes of words
+  if (e != cudaSuccess) return launched(e);
+  k_recur_timeout<<<1, 32, 0, s>>>(reinterpret_cast<const ulonglong2*>(base + 256),
+                                   reinterpret_cast<int*>(base), polls);
+  return launched(cudaGetLastError());
 }

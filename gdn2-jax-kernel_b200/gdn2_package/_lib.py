@@ -65,6 +65,7 @@ SIGNATURES = {
     "gdn2_recur_kept_floats": (_sz, [_i] * 4),
     "gdn2_recur_workspace_bytes": (_sz, [_i] * 4),
     "gdn2_recur_fwd": (_i, [_i] + [_vp] * 12 + [_sz] + [_i] * 4 + [_vp]),
+    "gdn2_selftest_recur_timeout": (_i, [_vp, _sz, _i, _vp]),
     "gdn2_recur_bwd": (_i, [_i] + [_vp] * 15 + [_sz] + [_i] * 4 + [_vp]),
     "gdn2_diag_read": (_i, [_vp, _sz, _vp, _i, ctypes.POINTER(ctypes.c_int),
                             ctypes.POINTER(ctypes.c_float)]),

@@ -8,7 +8,7 @@ from conftest import cuda_ok
 pytestmark = [pytest.mark.gpu, pytest.mark.skipif(not cuda_ok(), reason="needs a CUDA device")]
 
 from int8_ref import assert_close, linrec64, values64  # noqa: E402
-from gdn2_package import (gdn2_fwd, gdn2_linear_recurrence,  # noqa: E402
+from gdn2_package import (_lib, gdn2_fwd, gdn2_linear_recurrence,  # noqa: E402
                           gdn2_linear_recurrence_backward, gdn2_linear_recurrence_trainable,
                           gdn2_linear_recurrence_with_residuals)
 
@@ -308,6 +308,21 @@ def test_captured_and_replayed(T):
         g.replay()
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for a, b in zip(want, out))
+
+
+def test_a_wait_that_runs_out_is_reported(monkeypatch):
+    """A bounded wait for a word that nothing publishes gives up, is in the
+    status, and the same scratch and context serve the next call."""
+    lib, stream = _lib.load(), torch.cuda.current_stream().cuda_stream
+    ws = torch.empty(lib.gdn2_recur_workspace_bytes(1, 200, 1, 64), dtype=torch.uint8, device="cuda")
+    assert lib.gdn2_selftest_recur_timeout(ws.data_ptr(), ws.numel(), 64, stream) == _lib.OK
+    assert _lib.workspace_status(ws, stream) == _lib.STATUS_WAIT_TIMEOUT
+    with pytest.raises(_lib.Gdn2Error, match="timed out"):
+        _lib.check_status(ws, stream, "recurrence", synced=True)
+    monkeypatch.setattr(_lib, "CHECK_STATUS", "always")
+    x, do, dh = make(1, 200, 1, 64, seed=21)
+    check(x, do, dh)
+    assert _lib.LAST_STATUS == 0
 
 
 def test_long_sequence_of_slow_decay():

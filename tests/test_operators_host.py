@@ -91,6 +91,12 @@ def test_recurrence_entry_points_refuse():
     assert bwd(n=16) == _lib.ERR_WORKSPACE
 
 
+def test_timeout_selftest_refuses():
+    lib = _lib.load()
+    for ws, n, polls in ((None, 4096, 8), (P, 512, 8), (P, 4096, 0)):
+        assert lib.gdn2_selftest_recur_timeout(ws, n, polls, None) == _lib.ERR_INVALID
+
+
 def test_recurrence_sizes():
     lib = _lib.load()
     assert lib.gdn2_recur_kept_floats(2, 65, 3, 64) == 2 * 2 * 3 * 64
