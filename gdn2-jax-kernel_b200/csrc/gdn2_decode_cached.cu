@@ -7,8 +7,9 @@
 // What bounds it is the instructions of taking every code apart and putting it
 // together again: 16 a value, issued at 2.7 of 4 a cycle.  One token for 256 rows
 // x 8 heads of 128 takes 22.6 us, 48% of the copy rate (1024 rows: 86 us, 51%);
-// one row 4.3 us, all of it latency.  Four tokens a call take 67 us, a
-// quarter less than four calls; 16 warps a CTA made that 103 us (more partial sums).
+// one row 4.3 us, all of it latency.  Four tokens a call take 69 us, a
+// quarter less than four calls; 16 warps a CTA made that half as long again (more
+// partial sums).
 //
 // One CTA per (row, head).  The head's codes and scales (17 KB, contiguous) come
 // to shared memory by asynchronous copies, so the bytes in flight do not cost
@@ -84,7 +85,10 @@ k_decode_cached(const T* __restrict__ q, const T* __restrict__ k, const T* __res
                 G = Shape<D>::G;
   __shared__ __align__(16) int8_t scodes[D * D];
   __shared__ __align__(16) float sscales[D * G];
-  __shared__ float4 vec[ONE ? 1 : 2][D];   // W, qg, kg, e^{gc_last} of a token
+  // W, qg, kg, e^{gc_last} of a token.  Three tokens: the update of token t - 1 reads
+  // its own, with no synchronisation of the CTA between it and the put of token t + 1.  (Two, put after
+  // the first synchronisation: 69 to 71 us instead of 69 for the four tokens above.)
+  __shared__ float4 vec[ONE ? 1 : 3][D];
   __shared__ float red[ONE ? 1 : 2][D / 32], su[ONE ? 1 : 2][D];
   __shared__ __align__(16) float2 part[NW][D];   // per warp: W^T h, qg^T h
   __shared__ __align__(16) float snew[D];
@@ -116,15 +120,15 @@ k_decode_cached(const T* __restrict__ q, const T* __restrict__ k, const T* __res
     tb = to_f<T>(b[off + tid]);
     tg = to_f<T>(g[off + tid]);
   };
-  auto put = [&](int buf) {
+  auto put = [&](int buf, int at) {   // at: of vec; buf: of red and su
     if (gates) {
       tw = gate_act(tw, kGateW);
       tb = gate_act(tb, kGateB);
       tg = gate_act(tg, kGateG);
     }
     const float eg = expf(tg);
-    vec[buf][tid] = make_float4(san(a1 * (tb * tk * eg), clip), san(tq * eg, clip), san(tk, clip),
-                                expf(san(tg, clip)));
+    vec[at][tid] = make_float4(san(a1 * (tb * tk * eg), clip), san(tq * eg, clip), san(tk, clip),
+                               expf(san(tg, clip)));
     su[buf][tid] = san(a1 * (tw * tv), clip);
     float qk = tq * tk;
 #pragma unroll
@@ -135,7 +139,7 @@ k_decode_cached(const T* __restrict__ q, const T* __restrict__ k, const T* __res
   // a token is loaded a whole token before it is put, so that nothing waits for it
   if (tid < D) {
     load(off);
-    put(0);
+    put(0, 0);
     if (!ONE && T_ > 1) load(off + (size_t)H * D);
   }
 
@@ -173,12 +177,13 @@ k_decode_cached(const T* __restrict__ q, const T* __restrict__ k, const T* __res
     }
   }
 
+  int at = 0;   // of token t in vec
   for (int t = 0; t < (ONE ? 1 : T_); ++t, off += (size_t)H * D) {
-    const int buf = ONE ? 0 : t & 1;
+    const int buf = ONE ? 0 : t & 1, after = ONE || at == 2 ? 0 : at + 1;
     float2 wa[4] = {}, qa[4] = {};
 #pragma unroll
     for (int r = 0; r < R; ++r) {
-      float4 z = vec[buf][row_of(r)];
+      float4 z = vec[at][row_of(r)];
       if constexpr (ONE) {
         const float x = scale_of(row_of(r));
         convert8(word_of(row_of(r)), s[r & 3]);
@@ -206,7 +211,7 @@ k_decode_cached(const T* __restrict__ q, const T* __restrict__ k, const T* __res
         *reinterpret_cast<float4*>(&part[warp][cl * 8 + 2 * i]) =
             make_float4(wa[i].x, qa[i].x, wa[i].y, qa[i].y);
     if (!ONE && t + 1 < T_ && tid < D) {
-      put(buf ^ 1);
+      put(buf ^ 1, after);
       if (t + 2 < T_) load(off + 2 * (size_t)H * D);
     }
     __syncthreads();
@@ -232,7 +237,7 @@ k_decode_cached(const T* __restrict__ q, const T* __restrict__ k, const T* __res
       float top = 0.f;
 #pragma unroll
       for (int r = 0; r < R; ++r) {
-        const float4 z = vec[buf][row_of(r)];
+        const float4 z = vec[at][row_of(r)];
         update8(s[r], z.w, z.z, vn);
         top = max_abs(top, top8(s[r]));
       }
@@ -242,6 +247,7 @@ k_decode_cached(const T* __restrict__ q, const T* __restrict__ k, const T* __res
 #pragma unroll
           for (int i = 0; i < 4; ++i) s[r][i] = make_float2(san(s[r][i].x, clip), san(s[r][i].y, clip));
     }
+    at = after;
   }
 
   if (to < 0) return;

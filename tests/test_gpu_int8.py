@@ -442,3 +442,27 @@ def test_prompt_cache_and_generation_together():
     o8, h8 = gdn2_pallas_forward(*tail, scale, gdn2_state_read(cache, [1, 2]))
     o32, h32 = gdn2_pallas_forward(*tail, scale, h_f)
     assert rel(o8, o32) < 0.02 and rel(h8, h32) < 0.02
+
+
+@pytest.mark.parametrize("T,H,D,dtype", [(3, 4, 128, torch.bfloat16), (4, 8, 128, torch.float32),
+                                         (5, 5, 64, torch.float32), (17, 2, 64, torch.bfloat16),
+                                         (64, 2, 128, torch.float32)])
+def test_several_tokens_of_a_full_batch(T, H, D, dtype):
+    """More CTAs than the GPU holds and many tokens a call, so that the warps of a
+    CTA drift apart: every run gives the same bits, those of the float64 tokens."""
+    B = 512
+    args, scale = tokens(B, T, H, D, dtype, seed=63 + T)
+    cache = Gdn2StateCache(2 * B, H, D)
+    gdn2_state_write(cache, states(B, H, D, seed=15), list(range(B)))
+    src = torch.arange(B, device="cuda", dtype=torch.int32)
+    dst = src + B
+    o = gdn2_decode_cached(*args, scale, cache, src, dst)
+    h = gdn2_state_read(cache, dst)
+    for _ in range(10):
+        cache.codes[B:].zero_()
+        assert torch.equal(o, gdn2_decode_cached(*args, scale, cache, src, dst))
+        assert torch.equal(h, gdn2_state_read(cache, dst))
+    rows = [0, 1, 200, 293, 511]
+    o_r, h_r = oracle([t[rows] for t in args], scale, gdn2_state_read(cache, rows))
+    assert rel(o[rows], o_r) < 1e-5
+    check_state(h[rows], h_r)
