@@ -25,10 +25,15 @@ GROUP = 64         # values that share a scale
 _MAX_TENSORS = 8   # of one launch (GDN2_INT8_MAX_TENSORS)
 
 
-def _operand(t, dev, dtype):
-    """``t`` on ``dev`` in ``dtype``, contiguous and on a 16-byte boundary."""
+def _operand(t, dev, dtype, waits=False):
+    """``t`` on ``dev`` in ``dtype``, contiguous and on a 16-byte boundary.
+
+    A copy from pinned host memory is waited for, so that the caller may refill it
+    after the call, unless the call ``waits`` for its stream anyway (it returns
+    results on the host) or is being captured (its replays read the memory)."""
     if t.dtype is not dtype or t.device != dev:
-        t = t.to(device=dev, dtype=dtype, non_blocking=True)
+        t = t.to(device=dev, dtype=dtype, non_blocking=waits or t.is_cuda
+                 or torch.cuda.is_current_stream_capturing())
     if not t.is_contiguous():
         t = t.contiguous()
     return t.clone() if t.data_ptr() % 16 else t

@@ -59,7 +59,9 @@ class _Call:
         bf16 = vt is wt is gt is torch.bfloat16
         cdt = torch.bfloat16 if bf16 else torch.float32
         self.code = (_lib.BF16 if bf16 else _lib.F32) | (_lib.GATES_RAW if gates == "raw" else 0)
-        self.v, self.w, self.g = _operand(v, dev, cdt), _operand(w, dev, cdt), _operand(g, dev, cdt)
+        host = self.on_host
+        self.v, self.w = _operand(v, dev, cdt, host), _operand(w, dev, cdt, host)
+        self.g = _operand(g, dev, cdt, host)
         self.h0 = self.h0_dtype = None
         if h0 is not None:
             if not isinstance(h0, torch.Tensor):
@@ -67,7 +69,7 @@ class _Call:
             if h0.shape != (B, H, D):
                 raise _fwd.Gdn2ShapeError(f"h0 must be {(B, H, D)}; got {tuple(h0.shape)}")
             self.h0_dtype = h0.dtype
-            self.h0 = _operand(h0, dev, torch.float32)
+            self.h0 = _operand(h0, dev, torch.float32, host)
 
 
 class Gdn2RecurrenceResiduals:
@@ -188,13 +190,13 @@ def gdn2_linear_recurrence_backward(residuals, dout, dh_final=None):
         dout = torch.as_tensor(dout)
     if dout.shape != r.shape:
         raise _fwd.Gdn2ShapeError(f"dout must be {r.shape}; got {tuple(dout.shape)}")
-    do, dh = _operand(dout, dev, torch.float32), None
+    do, dh = _operand(dout, dev, torch.float32, r.on_host), None
     if dh_final is not None:
         if not isinstance(dh_final, torch.Tensor):
             dh_final = torch.as_tensor(dh_final)
         if dh_final.shape != (B, H, D):
             raise _fwd.Gdn2ShapeError(f"dh_final must be {(B, H, D)}")
-        dh = _operand(dh_final, dev, torch.float32)
+        dh = _operand(dh_final, dev, torch.float32, r.on_host)
     lib = _lib.load()
     dv, dw, dg = torch.empty_like(r.g), torch.empty_like(r.g), torch.empty_like(r.g)
     dh0 = do.new_empty((B, H, D))

@@ -193,7 +193,8 @@ def gdn2_decode_cached(q, k, v, w, b, g, scale, cache, slots=None, out_slots=Non
                 raise _fwd.Gdn2ShapeError("a slot of out_slots is another row's slot")
     bf16 = dtypes.count(torch.bfloat16) == 6
     cdt = torch.bfloat16 if bf16 else torch.float32
-    x = [_operand(t, dev, cdt) for t in ts]   # copies live until the launch
+    on_host = not ts[0].is_cuda
+    x = [_operand(t, dev, cdt, on_host) for t in ts]   # copies live until the launch
     o = cache.scales.new_empty(shape)
     code = _lib.BF16 if bf16 else _lib.F32
     if _fwd.GATES == "raw":
@@ -203,4 +204,4 @@ def gdn2_decode_cached(q, k, v, w, b, g, scale, cache, slots=None, out_slots=Non
                         cache.scales.data_ptr(), _ptr(src), _ptr(dst), o.data_ptr(), B, T, H, D, S,
                         float(scale), float(_fwd.CLIP), _lib.raw_stream(dev.index))
     _lib.check(rc, "gdn2_decode_cached")
-    return o if ts[0].is_cuda else o.cpu()
+    return o.cpu() if on_host else o

@@ -466,3 +466,48 @@ def test_several_tokens_of_a_full_batch(T, H, D, dtype):
     o_r, h_r = oracle([t[rows] for t in args], scale, gdn2_state_read(cache, rows))
     assert rel(o[rows], o_r) < 1e-5
     check_state(h[rows], h_r)
+
+
+def hold():
+    """Keeps the current stream busy for some milliseconds, so that what a call
+    leaves to it has not run when the call returns."""
+    torch.cuda._sleep(20_000_000)
+
+
+def test_pinned_host_buffers_may_be_refilled_after_a_call():
+    """A call that returns nothing to the host has read its host arguments when it
+    returns, whatever its stream still has to do."""
+    h, x = states(2, 2, 64, seed=16).cpu().pin_memory(), torch.randn(3, 128).pin_memory()
+    want_h, want_x = values64(h).cuda(), values64(x)
+    cache = Gdn2StateCache(4, 2, 64)
+    args, scale = tokens(2, 1, 2, 64, seed=64)
+    want_o = gdn2_decode_cached(*args, scale, cache, [0, 1], [2, 3])
+    pinned = [t.cpu().pin_memory() for t in args[1:]]
+    at, to = (torch.tensor(t, device="cuda", dtype=torch.int32) for t in ([0, 1], [2, 3]))
+    hold()
+    gdn2_state_write(cache, h, at)   # (slots on the host would be waited for)
+    h.fill_(7.0)
+    hold()
+    kept = gdn2_checkpoint_pack(x)
+    x.fill_(7.0)
+    assert torch.equal(gdn2_state_read(cache, at), want_h)
+    assert torch.equal(gdn2_checkpoint_unpack(kept)[0], want_x)
+    cache.codes.zero_()
+    hold()
+    o = gdn2_decode_cached(args[0], *pinned, scale, cache, at, to)
+    for t in pinned:
+        t.fill_(7.0)
+    assert torch.equal(o, want_o)
+
+
+def test_captured_write_reads_its_pinned_states_when_it_is_replayed():
+    h = states(1, 2, 64, seed=17).cpu().pin_memory()
+    cache, at = Gdn2StateCache(2, 2, 64), torch.tensor([1], device="cuda", dtype=torch.int32)
+    gdn2_state_write(cache, h, at)
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        gdn2_state_write(cache, h, at)
+    h.mul_(-3.0)
+    g.replay()
+    assert torch.equal(gdn2_state_read(cache, at), values64(h).cuda())

@@ -358,3 +358,20 @@ def test_few_tokens(T):
     assert torch.equal(o, o1) and torch.equal(h, h1)
     check(x, do, dh)
     check(x, do, dh, int8=True)
+
+
+def test_pinned_host_buffers_may_be_refilled_after_a_call():
+    """Host arguments beside tensors on the GPU have been read when the call returns."""
+    x, do, dh = make(2, 70, 2, 64, seed=22)
+    o, h, res = gdn2_linear_recurrence_with_residuals(**x)
+    want = gdn2_linear_recurrence_backward(res, do, dh)
+    w, h0, d = (t.cpu().pin_memory() for t in (x["w"], x["h0"], do))
+    torch.cuda._sleep(20_000_000)   # some milliseconds, in which no copy starts
+    got = gdn2_linear_recurrence(x["v"], w, x["g"], h0)
+    w.fill_(7.0)
+    h0.fill_(7.0)
+    assert torch.equal(o, got[0]) and torch.equal(h, got[1])
+    torch.cuda._sleep(20_000_000)
+    got = gdn2_linear_recurrence_backward(res, d, dh)
+    d.fill_(7.0)
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
