@@ -70,11 +70,12 @@ __device__ __forceinline__ float max_abs3(float x, float y, float z) {
 
 // 127 / top for the codes, to 2^-22.5 of itself (what that leaves open the border
 // check decides).  Finite for every top: a group without a scale reads back as 0
-// or NaN whatever its codes.
+// or NaN whatever its codes.  The reciprocal is that of top / 16: of a top above
+// 2^126 it would lie below the normal range, with fewer bits.
 __device__ __forceinline__ float group_inv(float top) {
   float r;
-  asm("rcp.approx.f32 %0, %1;" : "=f"(r) : "f"(fmaxf(top, kInt8Tiny)));
-  return 127.f * r;
+  asm("rcp.approx.f32 %0, %1;" : "=f"(r) : "f"(0.0625f * fmaxf(top, kInt8Tiny)));
+  return 7.9375f * r;   // 127 / 16
 }
 // The stored scale, rounded once.
 __device__ __forceinline__ float group_scale(float top) {

@@ -511,3 +511,27 @@ def test_captured_write_reads_its_pinned_states_when_it_is_replayed():
     h.mul_(-3.0)
     g.replay()
     assert torch.equal(gdn2_state_read(cache, at), values64(h).cuda())
+
+
+def test_ties_and_their_neighbours_at_the_top_of_the_range():
+    """Groups whose largest value is next to float32's largest, where its
+    reciprocal is below the normal range: values on every half step and one
+    float32 step to either side of it, and one pair that such a reciprocal puts
+    on the wrong side (126.4999944 steps)."""
+    gen = torch.Generator().manual_seed(65)
+    tops = 2.0 ** (126 + 2 * torch.rand(2000, generator=gen, dtype=torch.float64))
+    tops = torch.cat([tops.float(), torch.tensor([2.0 ** 126, 2.0 ** 127, 2e38, 3e38,
+                                                  torch.finfo(torch.float32).max])])
+    half = (torch.arange(-127, 127) + 0.5)[1:-1].double() * tops.double().view(-1, 1) / 127.0
+    half = half.float()
+    far = torch.full_like(half, float("inf"))
+    x = torch.stack([half, torch.nextafter(half, far), torch.nextafter(half, -far)], 1)
+    x = x.view(len(tops), -1, 63)
+    x = torch.cat([x, tops.view(-1, 1, 1).expand(-1, x.shape[1], 1)], 2)
+    pair = torch.zeros(1, x.shape[1], 64)
+    pair[..., 0], pair[..., 1] = 3.3592143e38, 3.372492e38
+    x = torch.cat([x, pair]).cuda()
+    assert torch.isfinite(x).all()
+    kept = gdn2_checkpoint_pack(x)
+    codes, scales = pack64(x)
+    assert torch.equal(kept.codes[0].long(), codes) and torch.equal(kept.scales[0], scales)
