@@ -21,6 +21,8 @@
 //                         with int8 checkpoints 176 (79%) / 231 (74%)
 //     B1 T131072 H8 D128  float32  351 (93%) / 569 (101%)
 //                         bf16     299 (69%) / 428 (77%), int8 383 (65%) / 459 (63%)
+// Raw gates cost an exponential and a reciprocal for each gate: 153 / 346 us, with
+// int8 checkpoints 203 / 312, for the first; 357 / 703, 456 / 702 for the last.
 //
 // The tiles of a sequence run at the same time.  Each publishes its map before
 // it waits for anything.  Eight tiles in a row form a group; a tile walks from
@@ -124,14 +126,16 @@ __device__ __forceinline__ float ex2(float x) {
   return r;
 }
 constexpr float kLog2e = 1.4426950408889634f;
-// sigmoid(x) from e^{-|x|}, so that neither end overflows or cancels; subnormal
-// values stay (the gradient of a gate that is nearly shut).
-__device__ __forceinline__ float sig(float x) {
+// sigmoid(x) and its derivative sigmoid(x) sigmoid(-x) from e^{-|x|}, so that
+// neither end overflows or cancels (1 - sigmoid(x) does where a gate is open);
+// subnormal values stay (the gradient of a gate that is nearly shut).
+__device__ __forceinline__ float2 sig_slope(float x) {
   float e, r;
   asm("ex2.approx.f32 %0, %1;" : "=f"(e) : "f"(-kLog2e * fabsf(x)));
   asm("rcp.approx.f32 %0, %1;" : "=f"(r) : "f"(1.f + e));
-  return x > 0.f ? r : e * r;
+  return make_float2(x > 0.f ? r : e * r, e * r * r);
 }
+__device__ __forceinline__ float sig(float x) { return sig_slope(x).x; }
 // e^g, or from the pre-activation x of g = -softplus(x): sigmoid(-x).
 template <bool RAW>
 __device__ __forceinline__ float2 decay2(float2 g) {
@@ -586,16 +590,20 @@ __global__ void __launch_bounds__(256, 2) k_recur_bwd(const Args p) {
     for (int r = kRows - 1; r >= 0; --r) m = {mul2(a[r], m.a), mul2(a[r], add2(d[r], m.b))};
     joint.maps[back][lane] = flat(m);
   };
-  // v and w of row r of the present tile; behind the end anything: only states
-  // that nothing reads come of it
-  auto vw = [&](int r, float2& v, float2& w) {
+  // v, w and with raw gates dw/dx of row r of the present tile; behind the end
+  // anything: only states that nothing reads come of it
+  auto vw = [&](int r, float2& v, float2& w, float2& slope) {
     v = value2(ldraw(&st.v[r][2 * lane]));
     w = value2(ldraw(&st.w[r][2 * lane]));
     if constexpr (FROM8) {
       v = mul2(v, both(st.scale[2 * r]));
       w = mul2(w, both(st.scale[2 * r + 1]));
     }
-    w = gate2<RAW>(w);
+    if constexpr (RAW) {
+      const float2 x = sig_slope(w.x), y = sig_slope(w.y);
+      w = make_float2(x.x, y.x);
+      slope = make_float2(x.y, y.y);
+    }
   };
 
   Place now, next;
@@ -623,8 +631,8 @@ __global__ void __launch_bounds__(256, 2) k_recur_bwd(const Args p) {
     Map m = identity();
 #pragma unroll
     for (int r = 0; r < kRows; ++r) {
-      float2 v, w;
-      vw(r, v, w);
+      float2 v, w, slope;
+      vw(r, v, w, slope);
       x[r] = mul2(w, v);
       m = after({a[N][r], x[r]}, m);
     }
@@ -651,12 +659,12 @@ __global__ void __launch_bounds__(256, 2) k_recur_bwd(const Args p) {
       c = mul2(a[N][r], dh);
       if (r < z.rows) {
         const size_t i = z.i + 2 * lane + (size_t)r * p.HD;
-        float2 v, w;
-        vw(r, v, w);
+        float2 v, w, slope;
+        vw(r, v, w, slope);
         float2 dw = mul2(v, dh), dg = mul2(x[r], c);
         if constexpr (RAW) {
-          // d sigmoid(x) = w (1 - w); dg/dx = -sigmoid(x)
-          dw = make_float2(dw.x * (w.x * (1.f - w.x)), dw.y * (w.y * (1.f - w.y)));
+          dw = mul2(dw, slope);
+          // dg/dx = -sigmoid(x)
           const float2 g = value2(ldraw(static_cast<const T*>(p.g) + i));   // in L2
           dg = make_float2(-dg.x * sig(g.x), -dg.y * sig(g.y));
         }

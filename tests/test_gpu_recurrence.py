@@ -375,3 +375,27 @@ def test_pinned_host_buffers_may_be_refilled_after_a_call():
     got = gdn2_linear_recurrence_backward(res, d, dh)
     d.fill_(7.0)
     assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+@pytest.mark.parametrize("int8", [None, "int8"])
+@pytest.mark.parametrize("T", [40, 64, 150])
+def test_raw_gates_that_are_open_or_shut_have_their_slope(T, int8):
+    """dw = v dh sigmoid(x) sigmoid(-x) to float32's relative precision at both ends,
+    where sigmoid(x) itself is 1 to float32's precision from x = 17 on."""
+    gdn2_fwd.GATES = "raw"
+    x, do, dh = make(2, T, 2, 64, seed=23, raw=True)
+    at = torch.linspace(-80, 80, 64, device="cuda")   # a channel each
+    x["w"] = at.expand(2, T, 2, 64).contiguous()
+    x["g"].fill_(float("inf"))   # e^g of 0: dh is dout (and dh_final at the end)
+    _, _, res = gdn2_linear_recurrence_with_residuals(**x, checkpoint=int8)
+    _, dw, _, _ = gdn2_linear_recurrence_backward(res, do, dh)
+    v, w = (values64(x["v"]), values64(x["w"])) if int8 else (x["v"], x["w"])
+    d = do.clone()
+    d[:, -1] += dh   # one rounding, as in the kernel
+    w = w.double()
+    want = v.double() * d.double() * torch.sigmoid(w) * torch.sigmoid(-w)
+    # e^{-|x|} is off by 2^-22 and the rounding of its exponent, |x| 2^-23 at most with
+    # that of log2 e; 1 / (1 + e^{-|x|}) by 2^-22, twice; products by 2^-24, four of them
+    size = want.abs() * ((2 * w.abs() + 4 + 8 + 4) * 2.0 ** -24)
+    err = (dw.double() - want).abs()
+    assert bool((err <= size + 2.0 ** -140).all()), float((err / want.abs()).max())
