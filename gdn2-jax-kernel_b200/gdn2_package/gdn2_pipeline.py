@@ -13,6 +13,9 @@ the inputs, exactly like the reference (gdn2_pipeline.py:64-67).
 """
 from __future__ import annotations
 
+import contextlib
+import threading
+
 import torch
 
 from . import gdn2_bwd as _bwd
@@ -62,12 +65,35 @@ class _Gdn2Core(torch.autograd.Function):
         return dq, dk, dv, dw, db, dg, dh0, None, None
 
 
+# What a call of gdn2_fwd / gdn2_bwd reads from the module.
+_SETTINGS = ("BT", "BC", "CLIP", "EXACT_BT", "PAIR64", "MASKED_TAIL", "GATES")
+_settings_lock = threading.Lock()   # backward passes of several devices have a thread each
+
+
+def _settings():
+    return {n: getattr(_fwd, n) for n in _SETTINGS}
+
+
+@contextlib.contextmanager
+def _with_settings(saved):
+    """gdn2_fwd's settings as ``saved``, for one call."""
+    with _settings_lock:
+        now = _settings()
+        vars(_fwd).update(saved)
+        try:
+            yield
+        finally:
+            vars(_fwd).update(now)
+
+
 class _Gdn2CoreInt8(torch.autograd.Function):
     """_Gdn2Core that keeps q, k, v, w, b in 8 bits and recomputes the forward
-    from the restored values in the backward."""
+    from the restored values in the backward, under the forward's settings: the
+    kept w, b and g are what GATES said they are then."""
 
     @staticmethod
     def forward(ctx, q, k, v, w, b, g, h0, scale):
+        ctx.settings = _settings()
         o, h_final = _fwd.gdn2_pallas_forward(q, k, v, w, b, g, scale, h0)
         kept = gdn2_checkpoint_pack(q, k, v, w, b)
         ctx.scale, ctx.shapes, ctx.dtypes, ctx.on_host = scale, kept.shapes, kept.dtypes, kept.on_host
@@ -84,7 +110,8 @@ class _Gdn2CoreInt8(torch.autograd.Function):
         q, k, v, w, b = gdn2_checkpoint_unpack(
             Gdn2Checkpoint(list(zip(ctx.at, kept[::2], kept[1::2])), ctx.shapes, ctx.dtypes,
                            ctx.on_host))
-        grads = _bwd.gdn2_backward(q, k, v, w, b, g, ctx.scale, h0, do, dh_final)
+        with _with_settings(ctx.settings):
+            grads = _bwd.gdn2_backward(q, k, v, w, b, g, ctx.scale, h0, do, dh_final)
         return *grads, None
 
 

@@ -535,3 +535,32 @@ def test_ties_and_their_neighbours_at_the_top_of_the_range():
     kept = gdn2_checkpoint_pack(x)
     codes, scales = pack64(x)
     assert torch.equal(kept.codes[0].long(), codes) and torch.equal(kept.scales[0], scales)
+
+
+@pytest.mark.parametrize("D,bt,bc", [(64, 64, 16), (64, 256, 128), (256, 256, 128)])
+def test_gdn2_int8_backward_runs_under_the_settings_of_its_forward(D, bt, bc):
+    """Settings that change between the passes change nothing of the gradients, and
+    stay as they were changed."""
+    raw = D == 64   # a head dim of 256 takes activated gates alone
+    gdn2_fwd.BT, gdn2_fwd.BC, gdn2_fwd.CLIP = 64, 16, 0.5
+    gdn2_fwd.GATES = "raw" if raw else "activated"
+    inp = make_inputs(1, 128, 2, D, seed=66, h0_std=0.1)
+    args = [torch.as_tensor(inp[n]).cuda() for n in NAMES]
+    gen = torch.Generator().manual_seed(67)
+    if raw:
+        args[3:] = [torch.randn(1, 128, 2, D, generator=gen).cuda() for _ in range(3)]
+    do, dh = (torch.as_tensor(inp[n]).cuda() for n in ("dout", "dh_final"))
+    leaves = [t.clone().requires_grad_(True) for t in args]
+
+    def run():
+        return gdn2_pallas_forward_trainable(*leaves, inp["scale"], checkpoint="int8")
+
+    want = torch.autograd.grad(run(), leaves, (do, dh))
+    out = run()
+    gdn2_fwd.BT, gdn2_fwd.BC, gdn2_fwd.CLIP = bt, bc, 1e4
+    gdn2_fwd.GATES = "activated" if raw else "raw"
+    got = torch.autograd.grad(out, leaves, (do, dh))
+    for n, a, b in zip(NAMES, got, want):
+        assert torch.equal(a, b), n
+    assert (gdn2_fwd.BT, gdn2_fwd.BC, gdn2_fwd.CLIP) == (bt, bc, 1e4)
+    assert gdn2_fwd.GATES == ("activated" if raw else "raw")

@@ -180,3 +180,15 @@ def test_slot_arguments():
             slots(s, 2, 2, dev, "slots", True)
     with pytest.raises(bad, match="give slots"):
         slots(None, 3, 2, dev, "slots", True)
+
+
+def test_settings_come_back_after_a_call(monkeypatch):
+    from gdn2_package import gdn2_pipeline
+    saved = gdn2_pipeline._settings()
+    monkeypatch.setattr(gdn2_fwd, "GATES", "raw")
+    monkeypatch.setattr(gdn2_fwd, "CLIP", 7.0)
+    with pytest.raises(ZeroDivisionError):
+        with gdn2_pipeline._with_settings(saved):
+            assert gdn2_fwd.GATES == "activated" and gdn2_fwd.CLIP == 1e4
+            1 / 0
+    assert gdn2_fwd.GATES == "raw" and gdn2_fwd.CLIP == 7.0
