@@ -192,7 +192,9 @@ __device__ __forceinline__ Map unword(ulonglong2 v) {
 __device__ Map await(const ulonglong2* p, int* status, int polls = kPolls) {
   ulonglong2 v = peek(p);
   for (int i = 1; !__all_sync(0xffffffffu, there(v)); ++i) {
-    if (i >= polls || (i % 4096 == 0 && *(volatile int*)status)) {
+    // (lanes may read different status words: the warp leaves together or not at all)
+    if ((i >= polls || i % 4096 == 0) &&
+        __any_sync(0xffffffffu, i >= polls || *(volatile int*)status)) {
       if ((threadIdx.x & 31) == 0) atomicExch(status, 1);
       break;
     }
@@ -692,9 +694,10 @@ __global__ void __launch_bounds__(256, 2) k_recur_bwd(const Args p) {
   }
 }
 
-// One warp that waits for words that nothing publishes.
+// Two warps that wait for words that nothing publishes: one gives up after `polls`
+// polls, the other because of the first.
 __global__ void k_recur_timeout(const ulonglong2* words, int* status, int polls) {
-  await(words + threadIdx.x, status, polls);
+  await(words + threadIdx.x % 32, status, threadIdx.x < 32 ? polls : kPolls);
 }
 
 // One CTA for every place on the GPU, or one a tile where there are fewer.
@@ -850,7 +853,7 @@ extern "C" int gdn2_selftest_recur_timeout(void* workspace, size_t workspace_byt
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   const cudaError_t e = cudaMemsetAsync(base, 0, 768, s);   // the header and 512 bytes of words
   if (e != cudaSuccess) return launched(e);
-  k_recur_timeout<<<1, 32, 0, s>>>(reinterpret_cast<const ulonglong2*>(base + 256),
+  k_recur_timeout<<<1, 64, 0, s>>>(reinterpret_cast<const ulonglong2*>(base + 256),
                                    reinterpret_cast<int*>(base), polls);
   return launched(cudaGetLastError());
 }

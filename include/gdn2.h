@@ -351,9 +351,10 @@ int gdn2_selftest_gemm_tf32x3(const float* A, const float* B, float* D, int batc
  * nothing else is in flight, so the context stays usable. */
 int gdn2_selftest_wait_timeout(void* workspace, size_t workspace_bytes, int polls, void* stream);
 
-/* The same for the waits of the linear recurrence: one warp waits for a word of
- * the zeroed scratch that nothing publishes, gives up after `polls` polls and
- * records it in the status word.  workspace: at least 1024 bytes. */
+/* The same for the waits of the linear recurrence: two warps wait for a word of
+ * the zeroed scratch that nothing publishes.  One gives up after `polls` polls
+ * and records it in the status word, which ends the other's wait long before its
+ * own limit.  workspace: at least 1024 bytes. */
 int gdn2_selftest_recur_timeout(void* workspace, size_t workspace_bytes, int polls, void* stream);
 
 #ifdef __cplusplus

@@ -399,3 +399,17 @@ def test_raw_gates_that_are_open_or_shut_have_their_slope(T, int8):
     size = want.abs() * ((2 * w.abs() + 4 + 8 + 4) * 2.0 ** -24)
     err = (dw.double() - want).abs()
     assert bool((err <= size + 2.0 ** -140).all()), float((err / want.abs()).max())
+
+
+def test_a_wait_that_ran_out_ends_the_others():
+    """A wait of the full limit (about two seconds) ends within some thousand polls
+    of another's that ran out."""
+    lib, stream = _lib.load(), torch.cuda.current_stream().cuda_stream
+    ws = torch.empty(1024, dtype=torch.uint8, device="cuda")
+    for polls in (1, 64, 5000):
+        start, end = (torch.cuda.Event(enable_timing=True) for _ in range(2))
+        start.record()
+        assert lib.gdn2_selftest_recur_timeout(ws.data_ptr(), ws.numel(), polls, stream) == _lib.OK
+        end.record()
+        assert _lib.workspace_status(ws, stream) == _lib.STATUS_WAIT_TIMEOUT
+        assert start.elapsed_time(end) < 300
