@@ -294,10 +294,13 @@ k_decode_cached(const T* __restrict__ q, const T* __restrict__ k, const T* __res
       }
       m = around();
     }
-    // (m is finite here; the scale need not be the correctly rounded quotient that
-    // packed tensors promise, and its division was 3% of the instructions)
+    // (the scale need not be the correctly rounded quotient that packed tensors
+    // promise, and its division was 3% of the instructions; m is infinite only
+    // under a clip that is)
     if (cl % 8 < 4)
-      scales[(row0 + row_of(r0 + own)) * G + cl * 8 / kGroup] = m >= kInt8Tiny ? m * (1.f / 127.f) : 0.f;
+      scales[(row0 + row_of(r0 + own)) * G + cl * 8 / kGroup] =
+          m > 3.402823466e38f ? __uint_as_float(0x7fc00000u)
+          : m >= kInt8Tiny ? m * (1.f / 127.f) : 0.f;
     const float inv = group_inv(m);
 #pragma unroll
     for (int j = 0; j < 4; ++j) {

@@ -564,3 +564,31 @@ def test_gdn2_int8_backward_runs_under_the_settings_of_its_forward(D, bt, bc):
         assert torch.equal(a, b), n
     assert (gdn2_fwd.BT, gdn2_fwd.BC, gdn2_fwd.CLIP) == (bt, bc, 1e4)
     assert gdn2_fwd.GATES == ("activated" if raw else "raw")
+
+
+@pytest.mark.parametrize("T", [1, 2])
+def test_a_state_that_overflows_without_a_clip_reads_back_as_nan(T):
+    """CLIP of infinity: a group that holds an infinity is NaN throughout, as in a
+    pack or a write, and reads as 0 in the next decode; its neighbours are right."""
+    gdn2_fwd.CLIP = float("inf")
+    args, scale = tokens(1, T, 1, 128, seed=68)
+    for t in args:
+        t[:, :-1] = 0   # tokens before the last leave the zero state
+    q, k, v, w, b, g = args
+    k[0, -1, 0, 3], v[0, -1, 0, 5], w[0, -1, 0, 5] = 4.0, 3e38, 1.0
+    cache = Gdn2StateCache(2, 1, 128)
+    gdn2_decode_cached(*args, scale, cache, [0], [1])
+    h = gdn2_state_read(cache, [1])[0, 0]
+    assert torch.isnan(h[3, :64]).all()
+    h[3, :64] = 0
+    want = (k[0, -1, 0].double().unsqueeze(1) * (w * v)[0, -1, 0].double())
+    want[3, :64] = 0
+    check_state(h.view(1, 1, 128, 128), want.view(1, 1, 128, 128).cpu())
+    # the group counts as 0 from now on; in the other rows column 5 has rounded its
+    # neighbours away
+    more, _ = tokens(1, 1, 1, 128, seed=69)
+    o = gdn2_decode_cached(*more, scale, cache, [1], [-1])
+    h0 = gdn2_state_read(cache, [1])
+    h0[..., :64] = 0
+    o_r, _ = oracle(more, scale, h0, float("inf"))
+    assert rel(o[..., 6:], o_r[..., 6:]) < 1e-5
