@@ -23,10 +23,6 @@ constexpr float kInt8Tiny = 0x1p-100f;
 // 1.5 * 2^23: added to |y| < 2^22 it leaves rint(y) in the low bits
 constexpr float kCodeBias = 12582912.f;
 
-// |x| as an ordered integer: NaN above infinity above every finite value, so
-// an integer maximum keeps NaN (a float maximum would drop it).
-__device__ __forceinline__ unsigned abs_bits(float x) { return __float_as_uint(x) & 0x7fffffffu; }
-
 // max|x|, |y| that keeps a NaN.
 __device__ __forceinline__ float max_abs(float x, float y) {
   float r;

@@ -192,3 +192,16 @@ def test_settings_come_back_after_a_call(monkeypatch):
             assert gdn2_fwd.GATES == "activated" and gdn2_fwd.CLIP == 1e4
             1 / 0
     assert gdn2_fwd.GATES == "raw" and gdn2_fwd.CLIP == 7.0
+
+
+def test_bytes_that_the_recurrence_keeps():
+    """g, the states before every 64th token, and v and w or their 8-bit form."""
+    from gdn2_package.gdn2_recurrence import Gdn2RecurrenceResiduals
+    shape, n = (2, 130, 3, 64), 2 * 130 * 3 * 64
+    rest = (shape, None, False, 0, (torch.float32,) * 3, None)
+    g, kept = torch.zeros(shape), torch.zeros(2, 3, 3, 64)
+    full = Gdn2RecurrenceResiduals.with_tensors((*rest, False), g, kept, g.clone(), g.clone())
+    assert full.nbytes == 12 * n + 4 * kept.numel() and full.int8 is None
+    codes, scales = torch.zeros((2, *shape), dtype=torch.int8), torch.zeros(2, n // 64)
+    small = Gdn2RecurrenceResiduals.with_tensors((*rest, True), g, kept, codes, scales)
+    assert small.nbytes == 4 * n + 2 * n + 8 * (n // 64) + 4 * kept.numel() and small.v is None
