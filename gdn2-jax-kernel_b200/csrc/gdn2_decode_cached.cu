@@ -4,11 +4,14 @@
 // over the tokens of the call and stored as codes again.
 //
 // A step moves 2 x 17 KB a head at D = 128, against 2 x 64 KB for float32 states.
-// What bounds it is the instructions of taking every code apart and putting it
-// together again: 16 a value, issued at 2.7 of 4 a cycle.  One token for 256 rows
+// Taking every code apart and putting it together again costs 16 instructions a
+// value.  They are issued at 2.7 of 4 a cycle and no pipe is more than half busy:
+// a CTA loads a head, works and stores, one after the other, and three neighbours
+// do not fill its pauses (2048 CTAs are 3.5 waves).  One token for 256 rows
 // x 8 heads of 128 takes 22.6 us, 48% of the copy rate (1024 rows: 86 us, 51%);
 // one row 4.3 us, all of it latency.  Four tokens a call take 69 us, a
-// quarter less than four calls; 16 warps a CTA made that half as long again (more
+// quarter less than four calls (bytes ask for 13): a token after the first is two
+// passes over the state and two synchronisations, at two CTAs an SM; 16 warps a CTA made that half as long again (more
 // partial sums).
 //
 // One CTA per (row, head).  The head's codes and scales (17 KB, contiguous) come

@@ -2,8 +2,9 @@
 // consecutive values share one float32 scale,
 //     code = rint(127 x / max|x|)  (ties to even),   scale = max|x| / 127,
 //     value = code * scale.
-// The code is the correctly rounded one: it does not depend on the order or
-// the precision of the arithmetic that a caller compares with.  The error of a
+// The code is the correctly rounded one (except where the cached decode stores a
+// state): it does not depend on the order or the precision of the arithmetic that
+// a caller compares with.  The error of a
 // value is at most half a step, max|x| / 254.
 //   * A group whose largest |x| is below 2^-100 gets the scale 0 and reads back as
 //     zeros (its scale would leave the normal range).

@@ -14,14 +14,15 @@
 // row.  A thread folds its 8 tokens, the warps join their maps through shared
 // memory, and each thread walks its tokens again from the state that reaches
 // it: every global byte moves once.  What moves bounds the float32 kernels:
-// 16 bytes a value forward, 28 backward.  The bf16 and int8 ones move less and
-// are bound by latency and issue at 16 warps an SM (64 to 140 instructions for a
-// row of 64 channels).  Of the measured copy rate, forward / backward:
+// 16 bytes a value forward, 28 backward.  The bf16 and int8 ones move less for 64
+// to 140 instructions a row of 64 channels, issued at 1.6 to 2.3 of 4 a cycle: what
+// bounds them is the latency that 16 warps an SM, which wait for one another twice
+// a tile, do not hide.  Of the measured copy rate, forward / backward:
 //     B8 T8192 H6 D128    float32  133 us (92%) / 225 us (96%)
 //                         with int8 checkpoints 176 (79%) / 231 (74%)
 //     B1 T131072 H8 D128  float32  351 (93%) / 569 (101%)
 //                         bf16     299 (69%) / 428 (77%), int8 383 (65%) / 459 (63%)
-// Raw gates cost an exponential and a reciprocal for each gate: 153 / 346 us, with
+// Raw gates cost exponentials and reciprocals: 153 / 346 us, with
 // int8 checkpoints 203 / 312, for the first; 357 / 703, 456 / 702 for the last.
 //
 // The tiles of a sequence run at the same time.  Each publishes its map before
@@ -32,7 +33,8 @@
 // the first tiles of a group: 398 us instead of 350 for one sequence of
 // 131072 tokens and 1024 channels, float32 forward.)  The last tile of a group
 // publishes the state that enters the next.  So a sequence of n tiles is n / 16
-// dependent steps of 0.57 us, every state is formed by the same operations
+// dependent steps of 0.57 us (few chains wait for them: one of 131072 tokens and
+// 64 channels takes 76 / 86 us, 27% / 42% of the copy rate), every state is formed by the same operations
 // whatever ran first (results do not depend on timing), and a tile reads at most
 // 16 published words of 512 bytes.  A published word is 64 bits, (a, b) of one
 // channel, with the sign bit of a (never negative) set: zeroed memory is "not

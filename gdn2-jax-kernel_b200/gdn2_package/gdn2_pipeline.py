@@ -126,7 +126,9 @@ def gdn2_pallas_forward_trainable(q, k, v, w, b, g, scale, h0=None, recompute=Fa
 
     checkpoint="int8" keeps q, k, v, w, b in 8 bits (gdn2_checkpoint_pack) and
     g, h0 as they are, and recomputes the forward: the gradients are those at
-    the restored inputs, the outputs those of the inputs.
+    the restored inputs, the outputs those of the inputs.  ``recompute`` makes no
+    difference then.  The backward runs under the settings of gdn2_fwd (BT, CLIP,
+    GATES and the others) that its forward had.
     """
     if checkpoint not in (None, "int8"):
         raise _fwd.Gdn2ShapeError(f"checkpoint={checkpoint!r}: None or 'int8'")

@@ -11,7 +11,9 @@ and drops what is written to it, so it pads a batch.  Slots given on the host
 are checked there; slots on the device are checked by the kernels, which give
 NaN for a row they refuse.
 
-Each store rounds a state value by at most 1/254 of the largest of its group.
+Each store rounds a state value by at most 1/254 of the largest of its group
+(``gdn2_decode_cached`` by 3e-5 of a step more: it takes the nearest code by
+float32 arithmetic, where ``gdn2_state_write`` decides it exactly).
 ``gdn2_decode_cached`` rounds once a call, whatever T is: the state is float32
 between the call's tokens.  A decay or an update below half a step of its group
 is lost in that rounding, so sequences that must remember over very many single
@@ -154,7 +156,8 @@ def gdn2_decode_cached(q, k, v, w, b, g, scale, cache, slots=None, out_slots=Non
     """``gdn2_decode`` from the states in ``slots`` into ``out_slots`` of the
     cache (the same slots by default; slot b for row b where neither is given).
 
-    q..g (B, T, H, D) with T as small as 1; returns o (B, T, H, D) float32.
+    q..g (B, T, H, D) with T as small as 1 and D 64 or 128 (states of 256
+    are read for ``gdn2_pallas_forward``); returns o (B, T, H, D) float32.
     Several rows may start from one slot, each with a destination of its own (a
     shared prefix).  A destination must not be another row's source or
     destination: the host refuses such slots where it has them, the kernel gives

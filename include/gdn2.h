@@ -33,7 +33,8 @@ extern "C" {
 
 enum { GDN2_F32 = 0, GDN2_BF16 = 1 };
 /* OR-ed into the dtype argument of gdn2_fwd / gdn2_bwd / gdn2_fwd_noalloc /
- * gdn2_decode / gdn2_decode_cached / gdn2_recur_fwd / gdn2_recur_bwd: w, b, g are pre-activations and the kernels apply
+ * gdn2_decode / gdn2_decode_cached / gdn2_recur_fwd / gdn2_recur_bwd: w, b, g
+ * are pre-activations and the kernels apply
  * w = sigmoid(w), b = sigmoid(b), g = -softplus(g) as they load them (the
  * activations the reference leaves to its caller, README.md:60-68).
  * gdn2_bwd then returns dw, db, dg with respect to the pre-activations.  The
@@ -282,8 +283,10 @@ int gdn2_state_read(int dtype, const void* codes, const float* scales, const int
  * slots lie outside the cache, or whose destination is another row's source or
  * destination, gets NaN outputs and stores nothing: its result would depend on
  * the order of blocks.  A state is taken as stored (the sanitiser acts as it is
- * written), a NaN scale as 0.  D is 64 or 128; codes and scales
- * are 16-byte aligned. */
+ * written), a NaN scale as 0.  It is stored by float32 arithmetic alone: a code
+ * may be the neighbour of the one above where 127 x / max|x| is within 3e-5 of a
+ * half, and the scale is within two roundings of max|x| / 127.  D is 64 or 128;
+ * codes and scales are 16-byte aligned. */
 int gdn2_decode_cached(int dtype, const void* q, const void* k, const void* v, const void* w,
                        const void* b, const void* g, void* codes, float* scales, const int* src,
                        const int* dst, float* o, int B, int T, int H, int D, int S, float scale,
